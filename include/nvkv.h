@@ -54,6 +54,7 @@ typedef struct CUstream_st* nvkv_stream_t; /* == cudaStream_t */
 #define NVKV_DEVERR_BLOCK_RANGE 2     /* block_tables entry >= num_blocks     */
 #define NVKV_DEVERR_POSITION_RANGE 3  /* positions[t] outside [0, max_pos)    */
 #define NVKV_DEVERR_SEQLEN 4          /* q_len > k_len or lengths > maxima    */
+#define NVKV_DEVERR_SLOT_ORDER 6      /* nvkv_rope_append: slots not ascending */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int nvkv_version(void);
@@ -220,6 +221,145 @@ int nvkv_paged_attention_fp8(const void* q, int64_t q_stride, int64_t num_q_toke
                              int num_kv_heads, int head_dim, int page_size, float softmax_scale,
                              int causal, int64_t prompt_kv_tokens, void* workspace,
                              size_t workspace_bytes, int dtype, nvkv_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions: both pair layouts, part of the head, any frequencies.
+ * Beside rotary_embedding.rs:11-70 (whole heads, half layout, plain
+ * frequencies), which nvkv_qknorm_rope computes at the reference's rounding
+ * points.
+ *
+ * nvkv_rope_frequencies (host): inv_freq[i], i < rot_dim / 2, in radians per
+ * position, and the factor a of cos and sin, from theta and a scaling (NULL:
+ * plain, theta^(-2i / rot_dim)):
+ *   LINEAR  plain / factor (positions interpolated);
+ *   NTK     plain with theta * factor^(rot_dim / (rot_dim - 2));
+ *   YARN    plain / factor for pairs that make fewer than beta_slow turns over
+ *           original_max_position, plain for those that make more than
+ *           beta_fast, a linear ramp over the pair index between; a = 0.1
+ *           ln(factor) + 1;
+ *   BANDS   plain / factor below low_freq_factor turns, plain above
+ *           high_freq_factor, a linear ramp in the turns between.
+ * attention_factor > 0 replaces a.  Both outputs are host memory.
+ *
+ * nvkv_rope: rows q [T, Hq, head_dim] and k [T, Hkv, head_dim] (token strides
+ * in elements; heads dense; either may have 0 heads and NULL pointers):
+ *   half layout:  pairs (x[i], x[i + rot_dim / 2]), i < rot_dim / 2
+ *   interleaved:  pairs (x[2i], x[2i + 1])
+ *   y0 = a (x0 cos - x1 sin), y1 = a (x1 cos + x0 sin) at the angle
+ *   positions[t] * inv_freq[i] (formed in f64); dims >= rot_dim are copied.
+ * f32 arithmetic, rounded once.  positions [T] int64, any sign: negated
+ * positions rotate back (with a = 1 the transposed rotation).  inv_freq: f64
+ * [rot_dim / 2] on the device.  An output may be its own input (same pointer
+ * and stride); any other overlap is refused.  rot_dim even, <= head_dim <=
+ * 1024.
+ * ---------------------------------------------------------------------- */
+#define NVKV_ROPE_PLAIN 0
+#define NVKV_ROPE_LINEAR 1
+#define NVKV_ROPE_NTK 2
+#define NVKV_ROPE_YARN 3
+#define NVKV_ROPE_BANDS 4
+
+typedef struct nvkv_rope_scaling {
+  int type;                      /* NVKV_ROPE_*                             */
+  double factor;                 /* >= 1 (all but PLAIN)                    */
+  int64_t original_max_position; /* YARN, BANDS                             */
+  double beta_fast, beta_slow;   /* YARN (32 and 1 are usual)               */
+  double low_freq_factor, high_freq_factor; /* BANDS (1 and 4 are usual)    */
+  double attention_factor;       /* > 0: used instead of the type's own     */
+} nvkv_rope_scaling;
+
+int nvkv_rope_frequencies(int rot_dim, double theta, const nvkv_rope_scaling* scaling,
+                          double* inv_freq, double* attn_factor);
+
+int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, void* q_out,
+              int64_t q_out_stride, void* k_out, int64_t k_out_stride, int64_t num_tokens,
+              int num_q_heads, int num_kv_heads, int head_dim, const int64_t* positions,
+              const double* inv_freq, int rot_dim, double attn_factor, int interleaved, int dtype,
+              nvkv_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Block-scaled FP8 (e4m3) KV pool ("fp8b"): one power-of-two scale for each
+ * block of 16 slots and kv head, filled by one launch that also rotates.  No
+ * counterpart in the reference; beside its store (kv_cache.rs:168-190),
+ * rotation and attention (attention.rs:37-75).
+ *
+ * Layout: k_cache / v_cache [num_blocks, page_size, Hkv, 128] e4m3 codes;
+ * kv_scale [num_blocks, Hkv, page_size / 16, 2] f32 (K, V), powers of two:
+ *   value = code * scale,  code = e4m3_rn(x / scale),
+ *   scale = 2^e, e the least integer >= -100 with amax <= 448 * 2^e, amax the
+ *   largest finite |x| of the block's rows (infinities take the largest
+ *   code, NaN stays NaN).
+ * Because scales are powers of two, a block that a larger row joins is
+ * re-encoded by shifting exponents: exact, but for codes that fall below
+ * e4m3's normal range.
+ *
+ * nvkv_rope_append: for each token t, in one launch,
+ *   q' = norm(q), k' = norm(k)   (RMSNorm per head with q_norm_w / k_norm_w
+ *        [128], both or neither);  nvkv_rope's rotation of q' and k' with
+ *   rot_dim % 8 == 0;  q_out [T, Hq, 128] = dtype(q'), and K, V appended at
+ *   slot_mapping[t] (negative: not stored; past the pool: not stored, recorded
+ *   as NVKV_DEVERR_SLOT_RANGE).
+ * kv_scale == NULL: k_cache / v_cache are the model-dtype pool [num_blocks,
+ *   page_size, Hkv, 128] and get dtype(k') and v.
+ * kv_scale != NULL: the fp8b pool.  K is normalised, rotated and rounded from
+ *   f64, so codes and scales are those of the formulas.  A block's rows are
+ *   appended in order: of a block that the call reaches, the rows below its
+ *   lowest slot are kept (re-encoded when the scale grows; a call that starts
+ *   at the block's first row starts the scale anew) and those above are no
+ *   longer valid.  The tokens that share a block must be neighbours in the
+ *   call with ascending slots, as nvkv_prepare_step and nvkv_decode_advance
+ *   lay them out; a token whose slot does not ascend from its neighbour's in
+ *   the same block is not stored, nor those after it in that block, and
+ *   NVKV_DEVERR_SLOT_ORDER is recorded.  A block that a call reaches again
+ *   after other blocks ends up with unspecified contents (no other block
+ *   does).
+ * q/k/v: [T, H, 128] with token strides (elements, multiples of 4), rows
+ * 8-byte aligned; num_q_heads may be 0 (q, q_out NULL).  q_out may be q.
+ *
+ * nvkv_load_kvcache_fp8b: k_out / v_out [n, Hkv, 128] = dtype(code * scale) of
+ * rows slots[i] (negative: zeros; past the pool: zeros, recorded).  f16
+ * outputs saturate at 65504.
+ *
+ * nvkv_paged_attention_fp8b: nvkv_paged_attention over an fp8b pool (paged
+ * only).  When max_seqlen_q * (Hq / Hkv) <= 32 every sequence runs on the
+ * decode kernel, up to that many query rows a sequence (a decode step, or a
+ * few tokens each); otherwise sequences with q_len == 1 do, and the keys of
+ * the others are dequantised into the workspace for the prefill kernel, so
+ * the caller passes prompt_kv_tokens >= the sum of their k_len (a prompt that
+ * does not fit is skipped and recorded as NVKV_DEVERR_SEQLEN).  Malformed
+ * sequences are skipped and recorded as in nvkv_paged_attention.  Products
+ * are exact in the codes: queries enter as three e4m3 pieces (12 significant
+ * bits), the softmax weights as three (2^-12 of a weight), sums in f32.  Calls
+ * that may overlap on the GPU need a workspace each.
+ * ---------------------------------------------------------------------- */
+#define NVKV_FP8B_BLOCK 16 /* slots that share a scale */
+
+int nvkv_rope_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, int64_t num_tokens, int num_q_heads,
+                     int num_kv_heads, int head_dim, const int64_t* positions,
+                     const double* inv_freq, int rot_dim, double attn_factor, int interleaved,
+                     const void* q_norm_w, const void* k_norm_w, float eps, void* q_out,
+                     void* k_cache, void* v_cache, float* kv_scale, const int64_t* slot_mapping,
+                     int64_t num_blocks, int page_size, int dtype, nvkv_stream_t stream);
+
+int nvkv_load_kvcache_fp8b(const void* k_cache, const void* v_cache, const float* kv_scale,
+                           const int64_t* slots, int64_t num_slots, int num_kv_heads, int head_dim,
+                           int64_t num_blocks, int page_size, void* k_out, void* v_out, int dtype,
+                           nvkv_stream_t stream);
+
+int nvkv_paged_attention_fp8b_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
+                                             int head_dim, int max_seqlen_q, int max_seqlen_k,
+                                             int64_t prompt_kv_tokens, size_t* bytes);
+
+int nvkv_paged_attention_fp8b(const void* q, int64_t q_stride, int64_t num_q_tokens,
+                              const void* k_cache, const void* v_cache, const float* kv_scale,
+                              int64_t num_blocks, void* out, const uint32_t* cu_seqlens_q,
+                              const uint32_t* cu_seqlens_k, const uint32_t* block_tables,
+                              int64_t block_table_stride, int num_seqs, int max_seqlen_q,
+                              int max_seqlen_k, int num_q_heads, int num_kv_heads, int head_dim,
+                              int page_size, float softmax_scale, int causal,
+                              int64_t prompt_kv_tokens, void* workspace, size_t workspace_bytes,
+                              int dtype, nvkv_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * nvkv_paged_attention without a workspace argument, for callers that cannot

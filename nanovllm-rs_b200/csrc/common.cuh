@@ -62,6 +62,11 @@ int encode_kv_tensor_map_u8(CUtensorMap* map, const void* base, int64_t row_byte
                             int64_t num_heads, int64_t num_rows, int64_t row_stride_bytes,
                             int box_rows);
 
+// Whether two arrays of `tokens` rows of 2-byte elements (token strides and row
+// lengths in elements) share memory, other than by being the same rows.
+bool rows_clash(const void* a, int64_t a_stride, int64_t a_row, const void* b, int64_t b_stride,
+                int64_t b_row, int64_t tokens);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Raises a kernel's dynamic shared-memory limit once per device (first call

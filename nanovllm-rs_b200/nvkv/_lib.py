@@ -31,6 +31,14 @@ DEVERR_BLOCK_RANGE = 2
 DEVERR_POSITION_RANGE = 3
 DEVERR_SEQLEN = 4
 DEVERR_PEER_TIMEOUT = 5
+DEVERR_SLOT_ORDER = 6
+
+ROPE_PLAIN = 0
+ROPE_LINEAR = 1
+ROPE_NTK = 2
+ROPE_YARN = 3
+ROPE_BANDS = 4
+FP8B_BLOCK = 16
 
 COMM_HANDLE_BYTES = 64
 COMM_MAX_RANKS = 8
@@ -41,6 +49,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
 
@@ -59,6 +68,14 @@ class StepSizes(ctypes.Structure):
                 ("num_need_logits", ctypes.c_int64), ("block_table_width", ctypes.c_int64),
                 ("max_seqlen_q", ctypes.c_int64), ("max_seqlen_k", ctypes.c_int64),
                 ("has_block_tables", ctypes.c_int)]
+
+
+class RopeScaling(ctypes.Structure):
+    """nvkv_rope_scaling: how the frequencies of nvkv_rope_frequencies are scaled."""
+    _fields_ = [("type", ctypes.c_int), ("factor", ctypes.c_double),
+                ("original_max_position", ctypes.c_int64), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double), ("low_freq_factor", ctypes.c_double),
+                ("high_freq_factor", ctypes.c_double), ("attention_factor", ctypes.c_double)]
 
 
 _seq = ctypes.POINTER(BlockSeq)
@@ -87,6 +104,17 @@ SIGNATURES = {
     "nvkv_paged_attention_fp8": [_p, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _i64,
                                  _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i64, _p,
                                  _sz, _i32, _p],
+    "nvkv_rope_frequencies": [_i32, _f64, ctypes.POINTER(RopeScaling), _p, ctypes.POINTER(_f64)],
+    "nvkv_rope": [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _i32, _p, _p, _i32,
+                  _f64, _i32, _i32, _p],
+    "nvkv_rope_append": [_p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _i32, _p, _p, _i32, _f64,
+                         _i32, _p, _p, _f32, _p, _p, _p, _p, _p, _i64, _i32, _i32, _p],
+    "nvkv_load_kvcache_fp8b": [_p, _p, _p, _p, _i64, _i32, _i32, _i64, _i32, _p, _p, _i32, _p],
+    "nvkv_paged_attention_fp8b_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32, _i64,
+                                                 ctypes.POINTER(_sz)],
+    "nvkv_paged_attention_fp8b": [_p, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i64, _i32,
+                                  _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i64, _p, _sz,
+                                  _i32, _p],
     "nvkv_rms_norm": [_p, _i64, _p, _i64, _p, _f32, _p, _i64, _i64, _i32, _i32, _p],
     "nvkv_silu_and_mul": [_p, _i64, _p, _i64, _i64, _i32, _i32, _p],
     "nvkv_decode_advance": [_i32, _i32, _p, _p, _i64, _i64, _p, _p, _p, _p, _p],

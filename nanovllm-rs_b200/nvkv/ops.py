@@ -11,7 +11,9 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._lib import DTYPE_BF16, DTYPE_F16, DTYPE_F32, NvkvError, ERR_INVALID_ARG, check, lib
+from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, ERR_INVALID_ARG, FP8B_BLOCK, NvkvError,
+                   ROPE_BANDS, ROPE_LINEAR, ROPE_NTK, ROPE_PLAIN, ROPE_YARN, RopeScaling, check,
+                   lib)
 
 _DT = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
@@ -44,6 +46,14 @@ def _row_view_ok(t: torch.Tensor) -> bool:
             return False
         exp *= t.size(d)
     return True
+
+
+def _same_device(*tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor on the current cuda device, whose stream the call uses."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        _need(t is None or (t.is_cuda and t.get_device() == dev),
+              "every tensor must be on the current cuda device")
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -222,6 +232,202 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         _ptr(block_tables), block_tables.size(1), B, int(max_seqlen_q), int(max_seqlen_k), hq, hkv,
         d, page, float(softmax_scale), 1 if causal else 0, int(prompt_kv_tokens),
         _ptr(workspace), ws_bytes, _dtype(q), _stream()))
+    return out
+
+
+ROPE_TYPES = {"plain": ROPE_PLAIN, "linear": ROPE_LINEAR, "ntk": ROPE_NTK, "yarn": ROPE_YARN,
+              "bands": ROPE_BANDS}
+
+
+def rope_frequencies(rot_dim: int, theta: float, scaling: str = "plain", factor: float = 1.0,
+                     original_max_position: int = 0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0, low_freq_factor: float = 1.0,
+                     high_freq_factor: float = 4.0,
+                     attention_factor: float = 0.0) -> Tuple[torch.Tensor, float]:
+    """(inv_freq f64 [rot_dim / 2] on the host, attention factor) of rotary
+    positions (nvkv_rope_frequencies): scaling is "plain", "linear", "ntk",
+    "yarn" or "bands"; move inv_freq to the device once and keep it."""
+    _need(scaling in ROPE_TYPES, f"scaling must be one of {sorted(ROPE_TYPES)}")
+    sc = RopeScaling(ROPE_TYPES[scaling], float(factor), int(original_max_position),
+                     float(beta_fast), float(beta_slow), float(low_freq_factor),
+                     float(high_freq_factor), float(attention_factor))
+    inv_freq = torch.empty(max(int(rot_dim) // 2, 1), dtype=torch.float64)
+    a = ctypes.c_double(1.0)
+    check(lib.nvkv_rope_frequencies(int(rot_dim), float(theta), ctypes.byref(sc), _ptr(inv_freq),
+                                    ctypes.byref(a)))
+    return inv_freq, a.value
+
+
+def _rope_args(positions: torch.Tensor, inv_freq: torch.Tensor, T: int) -> None:
+    _need(positions.dtype == torch.int64 and positions.is_contiguous() and
+          positions.numel() == T, "positions: contiguous int64 [T]")
+    _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
+          "inv_freq: contiguous f64 [rot_dim / 2]")
+
+
+def _stride0(t: Optional[torch.Tensor]) -> int:
+    """Token stride in elements (a single token's is its row length)."""
+    return 0 if t is None else t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
+
+
+def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+         inv_freq: torch.Tensor, attn_factor: float = 1.0, interleaved: bool = False,
+         q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None
+         ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotary positions of q [T, Hq, d] and k [T, Hkv, d] (nvkv_rope; token dims
+    may be strided, k may be None): the first 2 * inv_freq.numel() dims of every
+    head, half or interleaved pairs, f32 rounded once.  q_out / k_out default to
+    new tensors and may be q / k (in place).  Negated positions rotate back."""
+    for t in (q, k, q_out, k_out):
+        _need(t is None or (t.dim() == 3 and _row_view_ok(t) and t.dtype == q.dtype),
+              "q / k and their outputs: [T, H, d] of one dtype, rows dense")
+    T, hq, d = q.shape
+    _need(k is None or (k.size(0) == T and k.size(2) == d), "k must match q's tokens and head size")
+    _need(k is not None or k_out is None, "k_out without k")
+    _rope_args(positions, inv_freq, T)
+    if q_out is None:
+        q_out = torch.empty(T, hq, d, device=q.device, dtype=q.dtype)
+    if k is not None and k_out is None:
+        k_out = torch.empty(T, k.size(1), d, device=q.device, dtype=q.dtype)
+    _need(q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "output shape")
+    _same_device(q, k, q_out, k_out, positions, inv_freq)
+    check(lib.nvkv_rope(_ptr(q), _stride0(q), _ptr(k), _stride0(k), _ptr(q_out), _stride0(q_out),
+                        _ptr(k_out), _stride0(k_out), T, hq, 0 if k is None else k.size(1), d,
+                        _ptr(positions), _ptr(inv_freq), 2 * inv_freq.numel(), float(attn_factor),
+                        1 if interleaved else 0, _dtype(q), _stream()))
+    return q_out, k_out
+
+
+def _fp8b_pool(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: torch.Tensor) -> None:
+    _need(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and k_cache.dim() == 4 and
+          k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.shape == k_cache.shape,
+          "fp8b caches: contiguous uint8 [Nb, P, Hkv, 128]")
+    nb, page, hkv, _ = k_cache.shape
+    _need(kv_scale.dtype == torch.float32 and kv_scale.is_contiguous() and
+          page % FP8B_BLOCK == 0 and tuple(kv_scale.shape) == (nb, hkv, page // FP8B_BLOCK, 2),
+          "kv_scale: contiguous f32 [Nb, Hkv, P / 16, 2]")
+
+
+def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                positions: torch.Tensor, inv_freq: torch.Tensor, k_cache: torch.Tensor,
+                v_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                kv_scale: Optional[torch.Tensor] = None, attn_factor: float = 1.0,
+                interleaved: bool = False, q_norm_w: Optional[torch.Tensor] = None,
+                k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """q/k RMSNorm (with the weights) + rotary positions + append of k and v
+    [T, Hkv, 128] to a paged cache in one launch (nvkv_rope_append); returns the
+    rotated q [T, Hq, 128] (None without q).  The cache is the model-dtype pool
+    [Nb, P, Hkv, 128], or with kv_scale [Nb, Hkv, P / 16, 2] the block-scaled
+    e4m3 pool (uint8).  Tokens of one 16-slot block must be neighbours with
+    ascending slots."""
+    for t in (q, k, v, q_out):
+        _need(t is None or (t.dim() == 3 and _row_view_ok(t) and t.dtype == k.dtype),
+              "q, k, v: [T, H, 128] of one dtype, rows dense")
+    T, hkv, d = k.shape
+    _need(v.shape == k.shape and (q is None or (q.size(0) == T and q.size(2) == d)),
+          "q, k and v must match in tokens and head size")
+    _rope_args(positions, inv_freq, T)
+    _need(slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous() and
+          slot_mapping.numel() == T, "slot_mapping: contiguous int64 [T]")
+    if kv_scale is not None:
+        _fp8b_pool(k_cache, v_cache, kv_scale)
+    else:
+        _need(k_cache.dtype == k.dtype and v_cache.dtype == k.dtype and k_cache.dim() == 4 and
+              k_cache.is_contiguous() and v_cache.is_contiguous() and
+              v_cache.shape == k_cache.shape, "caches: contiguous [Nb, P, Hkv, 128] of k's dtype")
+    nb, page = k_cache.size(0), k_cache.size(1)
+    _need(k_cache.size(2) == hkv and k_cache.size(3) == d, "cache rows must match k")
+    for w in (q_norm_w, k_norm_w):
+        _need(w is None or (w.dtype == k.dtype and w.is_contiguous() and w.numel() == d),
+              "norm weights: [128] of k's dtype")
+    _need(q is not None or q_out is None, "q_out without q")
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    _need(q is None or (q_out.shape == q.shape and q_out.is_contiguous()), "q_out: contiguous")
+    _same_device(q, k, v, q_out, positions, inv_freq, k_cache, v_cache, kv_scale, slot_mapping,
+                 q_norm_w, k_norm_w)
+    check(lib.nvkv_rope_append(
+        _ptr(q), _stride0(q), _ptr(k), _stride0(k), _ptr(v), _stride0(v), T,
+        0 if q is None else q.size(1), hkv, d, _ptr(positions), _ptr(inv_freq),
+        2 * inv_freq.numel(), float(attn_factor), 1 if interleaved else 0, _ptr(q_norm_w),
+        _ptr(k_norm_w), float(eps), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(kv_scale),
+        _ptr(slot_mapping), nb, page, _dtype(k), _stream()))
+    return q_out
+
+
+def load_kvcache_fp8b(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: torch.Tensor,
+                      slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+                      k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None
+                      ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows `slots` [n] int64 of the block-scaled e4m3 pool as (k, v)
+    [n, Hkv, 128] bf16 / f16 (nvkv_load_kvcache_fp8b); negative slots give
+    zeros."""
+    _fp8b_pool(k_cache, v_cache, kv_scale)
+    nb, page, hkv, d = k_cache.shape
+    _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.is_contiguous(),
+          "slots: contiguous int64 [n]")
+    n = slots.numel()
+    if k_out is None:
+        k_out = torch.empty(n, hkv, d, device=k_cache.device, dtype=dtype)
+    if v_out is None:
+        v_out = torch.empty(n, hkv, d, device=k_cache.device, dtype=dtype)
+    for t in (k_out, v_out):
+        _need(tuple(t.shape) == (n, hkv, d) and t.is_contiguous() and t.dtype == k_out.dtype,
+              "outputs: contiguous [n, Hkv, 128] of one dtype")
+    _same_device(k_cache, v_cache, kv_scale, slots, k_out, v_out)
+    check(lib.nvkv_load_kvcache_fp8b(_ptr(k_cache), _ptr(v_cache), _ptr(kv_scale), _ptr(slots), n,
+                                     hkv, d, nb, page, _ptr(k_out), _ptr(v_out), _dtype(k_out),
+                                     _stream()))
+    return k_out, v_out
+
+
+def workspace_size_fp8b(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_seqlen_q: int,
+                        max_seqlen_k: int, prompt_kv_tokens: int = 0, head_dim: int = 128) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib.nvkv_paged_attention_fp8b_workspace_size(num_seqs, num_q_heads, num_kv_heads,
+                                                       head_dim, max_seqlen_q, max_seqlen_k,
+                                                       int(prompt_kv_tokens), ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention_fp8b(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         kv_scale: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                         cu_seqlens_k: torch.Tensor, block_tables: torch.Tensor,
+                         max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float,
+                         prompt_kv_tokens: int = 0, causal: bool = True,
+                         out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention over the block-scaled e4m3 pool (nvkv_paged_attention_fp8b).
+    prompt_kv_tokens: at least the sum of k_len over the q_len > 1 sequences,
+    needed when max_seqlen_q * Hq / Hkv > 32."""
+    _need(q.dim() == 3 and _row_view_ok(q), "q must be [T, Hq, D], rows dense")
+    _fp8b_pool(k_cache, v_cache, kv_scale)
+    _need(block_tables.dim() == 2 and block_tables.is_contiguous() and
+          block_tables.dtype in (torch.int32, torch.uint32), "block_tables: contiguous 32-bit [B, W]")
+    for t in (cu_seqlens_q, cu_seqlens_k):
+        _need(t.dtype in (torch.int32, torch.uint32) and t.is_contiguous() and t.numel() >= 1 and
+              t.numel() == cu_seqlens_q.numel(), "cu_seqlens: contiguous 32-bit [B + 1]")
+    T, hq, d = q.shape
+    nb, page, hkv = k_cache.size(0), k_cache.size(1), k_cache.size(2)
+    B = cu_seqlens_q.numel() - 1
+    _need(block_tables.size(0) >= B and k_cache.size(3) == d, "one block_tables row a sequence")
+    if out is None:
+        out = torch.empty(T, hq, d, device=q.device, dtype=q.dtype)
+    _need(out.shape == q.shape and out.is_contiguous() and out.dtype == q.dtype,
+          "out: contiguous, like q")
+    need = workspace_size_fp8b(B, hq, hkv, max_seqlen_q, max_seqlen_k, prompt_kv_tokens, d)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _same_device(q, k_cache, v_cache, kv_scale, cu_seqlens_q, cu_seqlens_k, block_tables, out,
+                 workspace)
+    check(lib.nvkv_paged_attention_fp8b(
+        _ptr(q), _stride0(q), T, _ptr(k_cache), _ptr(v_cache), _ptr(kv_scale), nb, _ptr(out),
+        _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), _ptr(block_tables), block_tables.size(1), B,
+        int(max_seqlen_q), int(max_seqlen_k), hq, hkv, d, page, float(softmax_scale),
+        1 if causal else 0, int(prompt_kv_tokens), _ptr(workspace), ws_bytes, _dtype(q),
+        _stream()))
     return out
 
 

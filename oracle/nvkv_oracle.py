@@ -457,7 +457,12 @@ E4M3_VALUES = _e4m3_table()
 def e4m3_encode(x) -> np.ndarray:
     """float32 -> e4m3 codes (uint8): round to nearest, ties to the even code,
     magnitudes above 448 saturate to 448 (the satfinite conversion)."""
-    x = np.asarray(x, np.float32).astype(np.float64)
+    return e4m3_encode64(np.asarray(x, np.float32))
+
+
+def e4m3_encode64(x) -> np.ndarray:
+    """e4m3_encode of f64 values, by one rounding."""
+    x = np.asarray(x, np.float64)
     a = np.minimum(np.abs(x), E4M3_MAX)
     e = np.floor(np.log2(np.maximum(a, 2.0 ** -9)))
     e = np.clip(e, -6, 8)  # exponent of the binade; below 2^-6 the subnormal step 2^-9
@@ -505,6 +510,87 @@ def dequantize_pages_fp8(cache, scales) -> np.ndarray:
     """[Nb, P, Hkv, D] codes + [Nb, Hkv, P] scales -> float32 values."""
     vals = e4m3_decode(cache)
     return (vals * np.transpose(scales, (0, 2, 1))[..., None]).astype(np.float32)
+
+
+# --------------------------------------------------------------------------
+# Rotary positions (any layout, part of the head, any frequencies) and the
+# block-scaled e4m3 pool: 16 slots and a kv head share a power-of-two scale.
+# No counterpart in the reference; the checker of nvkv_rope, nvkv_rope_append
+# and nvkv_paged_attention_fp8b, from the definitions in 64 bits.
+# --------------------------------------------------------------------------
+FP8B_BLOCK = 16
+FP8B_MIN_EXP = -100
+
+
+def rope_rotate(x, positions, inv_freq, attn_factor=1.0, interleaved=False) -> np.ndarray:
+    """x [T, H, d] rotated in f64: pairs (x[i], x[i + r/2]) or (x[2i], x[2i+1])
+    for i < r/2 = len(inv_freq), dims >= r copied."""
+    y = np.array(x, np.float64)
+    n = len(inv_freq)
+    ang = np.asarray(positions, np.float64)[:, None] * np.asarray(inv_freq, np.float64)
+    c, s = (attn_factor * np.cos(ang))[:, None], (attn_factor * np.sin(ang))[:, None]
+    i0 = slice(0, 2 * n, 2) if interleaved else slice(0, n)
+    i1 = slice(1, 2 * n, 2) if interleaved else slice(n, 2 * n)
+    a, b = y[..., i0].copy(), y[..., i1].copy()
+    y[..., i0], y[..., i1] = a * c - b * s, b * c + a * s
+    return y
+
+
+def head_rms_norm(x, w, eps) -> np.ndarray:
+    """Per-head RMSNorm in f64 (w None: identity); eps as the f32 that is passed."""
+    x = np.asarray(x, np.float64)
+    if w is None:
+        return x
+    var = np.mean(x * x, axis=-1, keepdims=True)
+    return x * (1.0 / np.sqrt(var + np.float64(np.float32(eps)))) * np.asarray(w, np.float64)
+
+
+def fp8b_exponent(amax) -> int:
+    """Least e >= -100 with amax <= 448 * 2^e."""
+    m, e = np.frexp(np.float64(amax))  # amax = m 2^e, 1/2 <= m < 1; 448 = 0.875 * 2^9
+    return max(int(e) - 9 + int(m > 0.875), FP8B_MIN_EXP) if amax > 0 else FP8B_MIN_EXP
+
+
+def append_fp8b(k, v, k_cache, v_cache, kv_scale, slot_mapping) -> None:
+    """Appends rows k, v [T, Hkv, D] (f64 values, K already rotated) to the
+    pool: caches [Nb, P, Hkv, D] uint8, kv_scale [Nb, Hkv, P / 16, 2]; a block's
+    tokens are neighbours with ascending slots."""
+    nb, P, hkv, D = k_cache.shape
+    slots = [int(s) for s in slot_mapping]
+    t = 0
+    while t < len(slots):
+        if slots[t] < 0:
+            t += 1
+            continue
+        end = t + 1
+        while end < len(slots) and slots[end] // FP8B_BLOCK == slots[t] // FP8B_BLOCK:
+            end += 1
+        page, at = slots[t] // P, slots[t] % P // FP8B_BLOCK
+        low = slots[t] % FP8B_BLOCK
+        for which, (x, cache) in enumerate(((k, k_cache), (v, v_cache))):
+            blk = cache[page, at * FP8B_BLOCK:(at + 1) * FP8B_BLOCK]
+            for h in range(hkv):
+                rows = np.asarray(x[t:end, h], np.float64)
+                mag = np.abs(rows)
+                e = fp8b_exponent(np.max(np.where(np.isfinite(mag), mag, 0.0), initial=0.0))
+                if low:
+                    old = int(np.frexp(kv_scale[page, h, at, which])[1]) - 1
+                    if old >= e:
+                        e = old
+                    else:
+                        blk[:low, h] = e4m3_encode64(e4m3_decode(blk[:low, h]) * 2.0 ** (old - e))
+                for j in range(t, end):
+                    row = np.clip(rows[j - t] * 2.0 ** -e, -E4M3_MAX, E4M3_MAX)
+                    codes = e4m3_encode64(np.where(np.isnan(row), 0.0, row))
+                    blk[slots[j] % FP8B_BLOCK, h] = np.where(np.isnan(row), 0x7F, codes)
+                kv_scale[page, h, at, which] = np.float32(2.0 ** e)
+        t = end
+
+
+def dequantize_pages_fp8b(cache, kv_scale, which) -> np.ndarray:
+    """[Nb, P, Hkv, D] codes -> f64 values (which: 0 K, 1 V)."""
+    sc = np.repeat(np.transpose(kv_scale[..., which], (0, 2, 1)), FP8B_BLOCK, axis=1)
+    return e4m3_decode(cache).astype(np.float64) * sc[..., None].astype(np.float64)
 
 
 # --------------------------------------------------------------------------
