@@ -115,6 +115,16 @@ size_t decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, i
 void decode_plan(int num_seqs, int num_kv_heads, int max_seqlen_k, bool fp8, int* chunk_tokens,
                  int* max_splits);
 int launch_paged_prefill(const AttnArgs& a);
+// fp8 pools: key offsets [num_seqs + 1] of the prompts' dequantised rows (0
+// rows for a decode row and for a prompt that is malformed or does not fit).
+int launch_prompt_rows(const uint32_t* cu_q, const uint32_t* cu_k, int num_seqs, int max_k,
+                       int64_t capacity, uint32_t* cu_kd, cudaStream_t stream);
+// Block-scaled fp8 pool (decode_fp8b.cu): sequences of at most q_cap query rows
+// (q_cap * group <= kFp8bMaxRows); others are left alone, or reported when
+// `all` says that every sequence should be such a one.
+constexpr int kFp8bMaxRows = 32;
+int launch_decode_fp8b(const AttnArgs& a, int q_cap, bool all);
+size_t decode_fp8b_bytes(int num_seqs, int hq, int hkv, int max_k, int q_cap);
 // Bytes of the prefill work plan (0 when max_seqlen_q <= 1); it sits in the
 // attention workspace after the decode scratch, at attention_plan_offset().
 size_t prefill_plan_bytes(int num_seqs, int max_seqlen_q);

@@ -226,6 +226,14 @@ F8Layout f8_layout(int num_seqs, int hq, int hkv, int max_q, int max_k, int64_t 
 }
 
 }  // namespace
+
+int launch_prompt_rows(const uint32_t* cu_q, const uint32_t* cu_k, int num_seqs, int max_k,
+                       int64_t capacity, uint32_t* cu_kd, cudaStream_t stream) {
+  fp8_prompt_rows_kernel<<<1, 1024, 0, stream>>>(cu_q, cu_k, num_seqs, max_k, capacity, cu_kd,
+                                                 device_error_word());
+  return check_cuda(cudaGetLastError(), "fp8 prompt rows launch");
+}
+
 }  // namespace nvkv
 
 extern "C" int nvkv_store_kvcache_fp8(const void* key, const void* value, void* k_cache,
@@ -369,9 +377,8 @@ extern "C" int nvkv_paged_attention_fp8(
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint32_t* cu_kd = reinterpret_cast<uint32_t*>(ws + L.cu_kd);
   int* err = device_error_word();
-  fp8_prompt_rows_kernel<<<1, 1024, 0, a.stream>>>(cu_seqlens_q, cu_seqlens_k, num_seqs,
-                                                    max_seqlen_k, prompt_kv_tokens, cu_kd, err);
-  rc = check_cuda(cudaGetLastError(), "fp8 prompt rows launch");
+  rc = launch_prompt_rows(cu_seqlens_q, cu_seqlens_k, num_seqs, max_seqlen_k, prompt_kv_tokens,
+                          cu_kd, a.stream);
   if (rc) return rc;
   const dim3 grid((unsigned)num_seqs, (unsigned)((max_seqlen_k + 63) / 64));
   if (dtype == NVKV_DTYPE_BF16)

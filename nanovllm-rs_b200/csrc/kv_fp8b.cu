@@ -73,88 +73,79 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Attention, the plain way: a CTA per (query row, kv head), its four warps over
-// the keys, f32 online softmax, one query head after the other.
-struct SimpleParams {
-  const void* q;
-  int64_t q_stride, num_q_rows;
-  const uint8_t *k, *v;
-  const float* scale;
-  void* out;
-  const uint32_t *cu_q, *cu_k, *bt;
-  int64_t bt_stride, num_blocks;
-  int num_seqs, max_k, hq, hkv, page, causal;
-  float sm;
-  int* err;
-};
-
+// Dequantises 64 keys of prompt blockIdx.x into rows cu_kd[b] + j of kbuf /
+// vbuf ([rows, Hkv, 128] in the dtype): a thread takes 16 codes.
 template <typename T>
-__global__ void __launch_bounds__(128) attend_fp8b_kernel(const SimpleParams p) {
-  __shared__ float so[4][kBD], sm_m[4], sm_l[4];
-  const uint32_t row = blockIdx.x;
-  const int kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int lo = 0, hi = p.num_seqs;  // the sequence of this row: cu_q[lo] <= row < cu_q[lo + 1]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (p.cu_q[mid] <= row) lo = mid;
-    else hi = mid;
+__global__ void __launch_bounds__(256)
+    dequant_prompt_fp8b_kernel(const uint8_t* __restrict__ k_cache,
+                               const uint8_t* __restrict__ v_cache, const float* __restrict__ scale,
+                               const uint32_t* __restrict__ cu_kd,
+                               const uint32_t* __restrict__ block_tables, int64_t bt_stride,
+                               int64_t num_blocks, int page, int hkv, T* __restrict__ kbuf,
+                               T* __restrict__ vbuf, int* err) {
+  const int b = blockIdx.x, j0 = blockIdx.y * 64;
+  const uint32_t ks = cu_kd[b];
+  const int len = (int)(cu_kd[b + 1] - ks);
+  if (j0 >= len) return;
+  // page_size is a multiple of 128: the 64 keys share a page
+  uint32_t pg = block_tables[(int64_t)b * bt_stride + j0 / page];
+  if ((int64_t)pg >= num_blocks) {
+    if (threadIdx.x == 0) record_error(err, NVKV_DEVERR_BLOCK_RANGE);
+    pg = 0;
   }
-  const uint32_t q0 = p.cu_q[lo], q1 = p.cu_q[lo + 1];
-  if (row < q0 || row >= q1) return;
-  const int q_len = (int)(q1 - q0), k_len = (int)(p.cu_k[lo + 1] - p.cu_k[lo]);
-  const bool bad = k_len > p.max_k || (int64_t)q1 > p.num_q_rows || (q_len > 1 && k_len < q_len);
-  if (bad || k_len <= 0) {
-    if (threadIdx.x == 0) record_error(p.err, NVKV_DEVERR_SEQLEN);
-    if (bad) return;
-  }
-  const int see = p.causal ? min(k_len, (int)(row - q0) + k_len - q_len + 1) : k_len;
-  const int g = p.hq / p.hkv, per = p.page / kBBlock;
-  for (int h = 0; h < g; ++h) {
-    const T* qr = static_cast<const T*>(p.q) + row * p.q_stride + (int64_t)(kvh * g + h) * kBD;
-    const uint2 raw = *reinterpret_cast<const uint2*>(qr + 4 * lane);
-    const float2 qa = DT<T>::to_f2(raw.x), qb = DT<T>::to_f2(raw.y);
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = warp; j < see; j += 4) {
-      uint32_t pg = p.bt[lo * p.bt_stride + j / p.page];
-      if ((int64_t)pg >= p.num_blocks) {
-        if (lane == 0) record_error(p.err, NVKV_DEVERR_BLOCK_RANGE);
-        pg = 0;
-      }
-      const int off = j % p.page;
-      const int64_t at = (((int64_t)pg * p.page + off) * p.hkv + kvh) * kBD + 4 * lane;
-      const float2 s2 = *reinterpret_cast<const float2*>(
-          p.scale + (((int64_t)pg * p.hkv + kvh) * per + off / kBBlock) * 2);
-      float kf[4], vf[4];
-      e4m3x4_f32(*reinterpret_cast<const uint32_t*>(p.k + at), kf);
-      e4m3x4_f32(*reinterpret_cast<const uint32_t*>(p.v + at), vf);
-      float s = qa.x * kf[0] + qa.y * kf[1] + qb.x * kf[2] + qb.y * kf[3];
+  const int per = page / kBBlock, off = j0 % page;
+  const int n = min(64, len - j0), chunks = hkv * 8;
+  for (int i = threadIdx.x; i < n * chunks * 2; i += blockDim.x) {
+    const int c = i % chunks, jj = i / chunks;
+    const int kv = jj >= n, j = kv ? jj - n : jj;
+    const int h = c >> 3;
+    const int64_t row = (int64_t)pg * page + off + j;
+    const uint4 w = *reinterpret_cast<const uint4*>((kv ? v_cache : k_cache) + row * hkv * kBD +
+                                                    (int64_t)c * 16);
+    const float s = scale[(((int64_t)pg * hkv + h) * per + (off + j) / kBBlock) * 2 + kv];
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint32_t o[8];
 #pragma unroll
-      for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= s2.x * p.sm;
-      const float mn = fmaxf(m, s);
-      const float al = exp2f(m - mn), e = exp2f(s - mn);
-      m = mn;
-      l = l * al + e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = o[i] * al + e * (vf[i] * s2.y);
+    for (int k = 0; k < 4; ++k) {
+      float f[4];
+      e4m3x4_f32(ws[k], f);
+      o[2 * k] = pack_value<T>(f[0] * s, f[1] * s);
+      o[2 * k + 1] = pack_value<T>(f[2] * s, f[3] * s);
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) so[warp][4 * lane + i] = o[i];
-    if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
-    __syncthreads();
-    float mx = -INFINITY;
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm_m[w]);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float acc = 0.f, ls = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(sm_m[w] - mu);
-      acc += so[w][threadIdx.x] * f;
-      ls += sm_l[w] * f;
-    }
-    static_cast<T*>(p.out)[((int64_t)row * p.hq + kvh * g + h) * kBD + threadIdx.x] =
-        DT<T>::from_f(ls == 0.f ? 0.f : acc / ls);
+    T* dst = (kv ? vbuf : kbuf) + ((int64_t)(ks + j0 + j) * chunks + c) * 16;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(dst + 8) = make_uint4(o[4], o[5], o[6], o[7]);
   }
+}
+
+// Query rows a sequence may have on the decode kernel: all sequences of a batch
+// whose longest fits, else single rows only.
+int short_rows(int hq, int hkv, int max_q) {
+  return (int64_t)max_q * (hq / hkv) <= kFp8bMaxRows ? max_q : 1;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Workspace: the decode kernel's partials and, at the same place (it is done
+// with them by then), the prefill kernel's region; for prompts then cu_kd
+// [num_seqs + 1] and their dequantised K and V rows.
+struct Layout {
+  size_t base, cu_kd, kbuf, vbuf, total;
+};
+Layout layout(int num_seqs, int hq, int hkv, int max_q, int max_k, int64_t prompt_rows) {
+  Layout L = {0, 0, 0, 0, 0};
+  if (num_seqs <= 0 || max_q <= 0) return L;
+  const int cap = short_rows(hq, hkv, max_q);
+  L.base = decode_fp8b_bytes(num_seqs, hq, hkv, max_k, cap);
+  L.total = L.base;
+  if (cap == max_q) return L;
+  L.base = std::max(L.base, attention_workspace_bytes(num_seqs, hq, hkv, max_q, max_k));
+  L.cu_kd = align256(L.base);
+  L.kbuf = align256(L.cu_kd + ((size_t)num_seqs + 1) * 4);
+  const size_t rows = (size_t)prompt_rows * hkv * kBD * 2;
+  L.vbuf = align256(L.kbuf + rows);
+  L.total = L.vbuf + rows;
+  return L;
 }
 
 }  // namespace
@@ -212,7 +203,9 @@ extern "C" int nvkv_paged_attention_fp8b_workspace_size(int num_seqs, int num_q_
   if (rc) return rc;
   if (prompt_kv_tokens < 0 || prompt_kv_tokens > 0x7fffffffLL)
     return set_error(NVKV_ERR_INVALID_ARG, "fp8b workspace_size: bad prompt_kv_tokens");
-  *bytes = 0;
+  *bytes = layout(num_seqs, num_q_heads, num_kv_heads, max_seqlen_q, max_seqlen_k,
+                  prompt_kv_tokens)
+               .total;
   return NVKV_OK;
 }
 
@@ -255,30 +248,75 @@ extern "C" int nvkv_paged_attention_fp8b(
     return set_error(NVKV_ERR_ALIGNMENT, "paged_attention_fp8b: metadata must be 4-byte aligned");
   if (!(softmax_scale > 0.f) || softmax_scale > 3e38f)
     return set_error(NVKV_ERR_INVALID_ARG, "paged_attention_fp8b: softmax_scale must be > 0");
-  SimpleParams p;
-  p.q = q;
-  p.q_stride = q_stride;
-  p.num_q_rows = num_q_tokens;
-  p.k = static_cast<const uint8_t*>(k_cache);
-  p.v = static_cast<const uint8_t*>(v_cache);
-  p.scale = kv_scale;
-  p.out = out;
-  p.cu_q = cu_seqlens_q;
-  p.cu_k = cu_seqlens_k;
-  p.bt = block_tables;
-  p.bt_stride = block_table_stride;
-  p.num_blocks = num_blocks;
-  p.num_seqs = num_seqs;
-  p.max_k = max_seqlen_k;
-  p.hq = num_q_heads;
-  p.hkv = num_kv_heads;
-  p.page = page_size;
-  p.causal = causal ? 1 : 0;
-  p.sm = softmax_scale * 1.4426950408889634f;
-  p.err = device_error_word();
-  const dim3 grid((unsigned)num_q_tokens, (unsigned)num_kv_heads);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == NVKV_DTYPE_BF16) attend_fp8b_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  else attend_fp8b_kernel<__half><<<grid, 128, 0, s>>>(p);
-  return check_cuda(cudaGetLastError(), "paged_attention_fp8b launch");
+  const int cap = short_rows(num_q_heads, num_kv_heads, max_seqlen_q);
+  const bool prompts = cap < max_seqlen_q;
+  if (prompts && prompt_kv_tokens == 0)
+    return set_error(NVKV_ERR_INVALID_ARG,
+                     "paged_attention_fp8b: max_seqlen_q * Hq / Hkv > 32 needs prompt_kv_tokens >= "
+                     "the prompts' total k_len");
+  const Layout L = layout(num_seqs, num_q_heads, num_kv_heads, max_seqlen_q, max_seqlen_k,
+                          prompt_kv_tokens);
+  if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
+    return set_error(NVKV_ERR_WORKSPACE, "paged_attention_fp8b: workspace missing or too small "
+                                         "(need " + std::to_string(L.total) + " bytes)");
+  AttnArgs a;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.num_q_rows = num_q_tokens;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.num_blocks = num_blocks;
+  a.kv_stride = (int64_t)num_kv_heads * head_dim;  // one byte a code
+  a.out = out;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.block_tables = block_tables;
+  a.bt_stride = block_table_stride;
+  a.num_seqs = num_seqs;
+  a.max_q = max_seqlen_q;
+  a.max_k = max_seqlen_k;
+  a.hq = num_q_heads;
+  a.hkv = num_kv_heads;
+  a.d = head_dim;
+  a.page = page_size;
+  a.scale = softmax_scale;
+  a.causal = causal ? 1 : 0;
+  a.ws = workspace;
+  a.ws_bytes = workspace_bytes;
+  a.dtype = dtype;
+  a.stream = reinterpret_cast<cudaStream_t>(stream);
+  a.k_scale = kv_scale;
+  rc = launch_decode_fp8b(a, cap, !prompts);
+  if (rc || !prompts) return rc;
+  // the others: dequantise their keys, then the contiguous prefill
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  uint32_t* cu_kd = reinterpret_cast<uint32_t*>(ws + L.cu_kd);
+  rc = launch_prompt_rows(cu_seqlens_q, cu_seqlens_k, num_seqs, max_seqlen_k, prompt_kv_tokens,
+                          cu_kd, a.stream);
+  if (rc) return rc;
+  const dim3 grid((unsigned)num_seqs, (unsigned)((max_seqlen_k + 63) / 64));
+  const auto* k8 = static_cast<const uint8_t*>(k_cache);
+  const auto* v8 = static_cast<const uint8_t*>(v_cache);
+  int* err = device_error_word();
+  if (dtype == NVKV_DTYPE_BF16)
+    dequant_prompt_fp8b_kernel<<<grid, 256, 0, a.stream>>>(
+        k8, v8, kv_scale, cu_kd, block_tables, block_table_stride, num_blocks, page_size,
+        num_kv_heads, reinterpret_cast<__nv_bfloat16*>(ws + L.kbuf),
+        reinterpret_cast<__nv_bfloat16*>(ws + L.vbuf), err);
+  else
+    dequant_prompt_fp8b_kernel<<<grid, 256, 0, a.stream>>>(
+        k8, v8, kv_scale, cu_kd, block_tables, block_table_stride, num_blocks, page_size,
+        num_kv_heads, reinterpret_cast<__half*>(ws + L.kbuf),
+        reinterpret_cast<__half*>(ws + L.vbuf), err);
+  rc = check_cuda(cudaGetLastError(), "fp8b dequant launch");
+  if (rc) return rc;
+  AttnArgs c = a;
+  c.k_cache = ws + L.kbuf;
+  c.v_cache = ws + L.vbuf;
+  c.k_scale = nullptr;
+  c.block_tables = nullptr;
+  c.bt_stride = 0;
+  c.num_blocks = prompt_kv_tokens;
+  c.cu_k = cu_kd;
+  return launch_paged_prefill(c);
 }
