@@ -12,13 +12,12 @@
 // compare them bit by bit.  q and the dtype pool use f32 and round once.
 //
 // Layout.  A CTA of 8 warps owns a window of W tokens: the cos / sin of those
-// tokens (and of the up to 15 that follow in the last one's block) go to shared
-// memory once; then warps take q rows (one per warp, lane l holds dims 4l ..
-// 4l + 3, pair partners meet by a shuffle) and K / V units.  A unit is one run
-// (the call's tokens of one block), one kv head, K or V: the warp holds all of
-// its up to 16 rows in registers (64 values a lane), so the maximum, the scale
-// and the codes come from one read.  The run belongs to the window of its first
-// token.  W = 1 for a decode step (a CTA per token: latency), up to 16 for
+// tokens go to shared memory once (f32 for q; f64 for the tokens of the runs,
+// up to 15 of them past the window); then warps take q rows and K / V units,
+// every pair in one lane.  A unit is one run (the call's tokens of one block),
+// one kv head, K or V: the warp holds all of its up to 16 rows in registers (64
+// values a lane), so the maximum, the scale and the codes come from one read.
+// The run belongs to the window of its first token.  W = 1 for a decode step (a CTA per token: latency), up to 16 for
 // prompts.  Bound by HBM for prompts (read qkv, write q and codes).
 #include <algorithm>
 #include <type_traits>
@@ -84,74 +83,160 @@ __device__ __forceinline__ void e4m3x4_f32(uint32_t w, float* f) {
   f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
 }
 
-template <typename R>
-struct CS;
-template <>
-struct CS<float> {
-  using V = float2;
+// A lane's dims of a rotated row: the chunks x[a], x[a + 1] and x[b], x[b + 1],
+// chosen so that every pair sits in one lane: pairs 2 lane and 2 lane + 1 of
+// either layout while lane < half / 2, dims that pass through behind them.
+struct LaneDims {
+  int a, b;
+  bool rot;
 };
-template <>
-struct CS<double> {
-  using V = double2;
-};
+__device__ __forceinline__ LaneDims lane_dims(int lane, int half, bool inter) {
+  LaneDims d;
+  d.rot = lane < half / 2;
+  d.a = d.rot && !inter ? 2 * lane : 4 * lane;  // half: pass-through dims 4 lane .. are >= 2 half
+  d.b = d.rot && !inter ? half + 2 * lane : 4 * lane + 2;
+  return d;
+}
 
-// Lane l's four dims 4l .. 4l + 3 of one head row, normalised (w != null) and
-// rotated by the table row cs, in R arithmetic.  Full warp.
-template <typename T, typename R, typename C>
-__device__ __forceinline__ void norm_rotate(const uint2 raw, const T* w, float eps, const C* cs,
-                                            int half, bool inter, int lane, R (&x)[4]) {
-  const float2 p0 = DT<T>::to_f2(raw.x), p1 = DT<T>::to_f2(raw.y);
-  x[0] = p0.x, x[1] = p0.y, x[2] = p1.x, x[3] = p1.y;
-  if (w) {
-    R ss = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+template <typename T, typename R>
+__device__ __forceinline__ void to_vals(uint32_t a, uint32_t b, R (&x)[4]) {
+  const float2 u = DT<T>::to_f2(a), v = DT<T>::to_f2(b);
+  x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
+}
+
+// x rotated by the lane's two pairs' (cos, sin)
+template <typename R, typename C>
+__device__ __forceinline__ void rotate(R (&x)[4], const C c0, const C c1, bool inter) {
+  const R p = x[0], q = inter ? x[1] : x[2], r = inter ? x[2] : x[1], s = x[3];
+  const R y0 = p * c0.x - q * c0.y, y1 = q * c0.x + p * c0.y;
+  const R y2 = r * c1.x - s * c1.y, y3 = s * c1.x + r * c1.y;
+  x[0] = y0;
+  x[1] = inter ? y1 : y2;
+  x[2] = inter ? y2 : y1;
+  x[3] = y3;
+}
+
+// Sums over the warp of N values a lane (N = 4 or 8): halving exchanges leave
+// row j's sum in the lanes with j in their upper bits (9 shuffles for 8 rows
+// instead of 40); row_lane(j) is one of them.
+template <int N>
+__device__ __forceinline__ int row_lane(int j) {
+  return N == 8 ? ((j >> 2) & 1) << 4 | ((j >> 1) & 1) << 3 | (j & 1) << 2
+                : ((j >> 1) & 1) << 4 | (j & 1) << 3;
+}
+template <int N, typename R>
+__device__ __forceinline__ R row_sums(R (&v)[N], int lane) {
+  int m = 16;
 #pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    const R inv = (R)1 / sqrt(ss / (R)kApD + (R)eps);
-    const uint2 wr = *reinterpret_cast<const uint2*>(w + 4 * lane);
-    const float2 w0 = DT<T>::to_f2(wr.x), w1 = DT<T>::to_f2(wr.y);
-    x[0] = x[0] * inv * (R)w0.x;
-    x[1] = x[1] * inv * (R)w0.y;
-    x[2] = x[2] * inv * (R)w1.x;
-    x[3] = x[3] * inv * (R)w1.y;
-  }
-  if (inter) {
-    if (4 * lane < 2 * half) {
-      const C c0 = cs[2 * lane], c1 = cs[2 * lane + 1];
-      const R a = x[0], b = x[2];
-      x[0] = a * (R)c0.x - x[1] * (R)c0.y;
-      x[1] = x[1] * (R)c0.x + a * (R)c0.y;
-      x[2] = b * (R)c1.x - x[3] * (R)c1.y;
-      x[3] = x[3] * (R)c1.x + b * (R)c1.y;
+  for (int n = N; n > 1; n >>= 1, m >>= 1) {
+    const bool up = lane & m;
+#pragma unroll
+    for (int j = 0; j < n / 2; ++j) {
+      const R keep = up ? v[j + n / 2] : v[j], give = up ? v[j] : v[j + n / 2];
+      v[j] = keep + __shfl_xor_sync(0xffffffffu, give, m);
     }
-  } else {
-    const int step = half >> 2;  // lanes between a pair's halves
-    const bool lo = lane < step, in = lane < 2 * step;
-    const int peer = lo ? lane + step : in ? lane - step : lane;
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const R y = __shfl_sync(0xffffffffu, x[i], peer);
-      if (in) {
-        const C c = cs[4 * (lo ? lane : peer) + i];
-        x[i] = lo ? x[i] * (R)c.x - y * (R)c.y : x[i] * (R)c.x + y * (R)c.y;
-      }
+  for (; m >= 1; m >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
+  return v[0];
+}
+
+// Up to N head rows (128 apart) of one token: norm, rotation, one rounding.
+template <typename T, int N>
+__device__ __forceinline__ void rows_f32(const T* src, T* dst, int n, const T* w, float eps,
+                                         const float2* cs, const LaneDims d, bool inter, int lane) {
+  uint32_t ra[N], rb[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const T* s = src + (j < n ? j : 0) * kApD;
+    ra[j] = *reinterpret_cast<const uint32_t*>(s + d.a);
+    rb[j] = *reinterpret_cast<const uint32_t*>(s + d.b);
+  }
+  const float2 c0 = d.rot ? cs[2 * lane] : make_float2(1.f, 0.f);
+  const float2 c1 = d.rot ? cs[2 * lane + 1] : make_float2(1.f, 0.f);
+  float inv = 1.f, wv[4] = {1.f, 1.f, 1.f, 1.f};
+  if (w) {
+    to_vals<T>(*reinterpret_cast<const uint32_t*>(w + d.a),
+               *reinterpret_cast<const uint32_t*>(w + d.b), wv);
+    float ss[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float x[4];
+      to_vals<T>(ra[j], rb[j], x);
+      ss[j] = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+    }
+    inv = 1.f / sqrtf(row_sums<N>(ss, lane) * (1.f / kApD) + eps);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float x[4];
+    to_vals<T>(ra[j], rb[j], x);
+    if (w) {
+      const float f = __shfl_sync(0xffffffffu, inv, row_lane<N>(j));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = x[i] * f * wv[i];
+    }
+    if (d.rot) rotate(x, c0, c1, inter);
+    if (j < n) {
+      *reinterpret_cast<uint32_t*>(dst + j * kApD + d.a) = DT<T>::from_f2(x[0], x[1]);
+      *reinterpret_cast<uint32_t*>(dst + j * kApD + d.b) = DT<T>::from_f2(x[2], x[3]);
     }
   }
 }
 
-template <typename T, bool kF8>
-__global__ void __launch_bounds__(kApThreads) rope_append_kernel(const AppendParams p) {
-  using R = typename std::conditional<kF8, double, float>::type;  // K's arithmetic
-  using C = typename CS<R>::V;
+// K rows j0 .. j0 + 7 of a run in f64: x[j] becomes the normalised, rotated
+// value rounded to odd.
+template <typename T>
+__device__ __forceinline__ void k_rows_f64(float (&x)[8][4], int n, const T* w, float eps,
+                                           const double2* cs, int half, const LaneDims d,
+                                           bool inter, int lane) {
+  double inv = 1.0, wv[4];
+  if (w) {
+    to_vals<T>(*reinterpret_cast<const uint32_t*>(w + d.a),
+               *reinterpret_cast<const uint32_t*>(w + d.b), wv);
+    double ss[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ss[j] = 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss[j] = fma((double)x[j][i], (double)x[j][i], ss[j]);
+    }
+    inv = rsqrt(row_sums<8>(ss, lane) * (1.0 / kApD) + (double)eps);  // for this lane's row
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j < n) {
+      double y[4] = {x[j][0], x[j][1], x[j][2], x[j][3]};
+      if (w) {
+        const double f = __shfl_sync(0xffffffffu, inv, row_lane<8>(j));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = y[i] * f * wv[i];
+      }
+      if (d.rot) rotate(y, cs[j * half + 2 * lane], cs[j * half + 2 * lane + 1], inter);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j][i] = f32_odd(y[i]);
+    }
+  }
+}
+
+// kWide: windows of several tokens (8 rows in flight a warp); else a decode
+// step's single tokens (4, so that eight warps share 32 heads).
+template <typename T, bool kF8, bool kWide>
+__global__ void __launch_bounds__(kApThreads, 2) rope_append_kernel(const AppendParams p) {
+  constexpr int kRows = kWide ? 8 : 4;
   extern __shared__ __align__(16) uint8_t smem[];
-  C* cs = reinterpret_cast<C*>(smem);  // [table tokens][half]
+  double2* cs64 = reinterpret_cast<double2*>(smem);  // [run tokens][half], fp8b pool
+  float2* cs = reinterpret_cast<float2*>(
+      smem + (kF8 ? (size_t)(p.window + kApBlock - 1) * p.half * sizeof(double2) : 0));
   __shared__ int64_t slot_s[kApTable + 1];  // slots of tokens w0 - 1 ..
-  __shared__ int lead_s[kApMaxWindow], len_s[kApMaxWindow], nrun_s, ntab_s;
+  __shared__ int lead_s[kApMaxWindow], len_s[kApMaxWindow], nrun_s, from_s, to_s;
   const int64_t w0 = (int64_t)blockIdx.x * p.window;
   const int n = (int)min((int64_t)p.window, p.num_tokens - w0);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // no memory access before this: the launch may overlap the kernel before it
-  pdl_wait();
-  if (warp == 0) {
+  pdl_wait();  // nothing is read or written before: the launch may overlap the kernel before it
+  for (int i = tid; i < n * p.half; i += kApThreads)
+    cs[i] = rope_cs(p.positions[w0 + i / p.half], p.inv_freq[i % p.half], (float)p.a);
+  if (warp == kApWarps - 1) {
     const int64_t t = w0 - 1 + lane;  // lane 0: the token before the window
     int64_t s = -1;
     if (t >= 0 && t < p.num_tokens && lane <= n + kApBlock - 1) {
@@ -172,101 +257,102 @@ __global__ void __launch_bounds__(kApThreads) rope_append_kernel(const AppendPar
       const uint32_t leads = __ballot_sync(0xffffffffu, in && s >= 0 && !same);
       // tokens from here on that continue this lane's run
       const uint32_t after = lane < 31 ? ~(joins >> (lane + 1)) : ~0u;
-      const int len = 1 + (__ffs(after) - 1);
+      const int len = __ffs(after);
       if (leads >> lane & 1) {
         const int r = __popc(leads & ((1u << lane) - 1));
         lead_s[r] = lane - 1;
         len_s[r] = len;
       }
       const int last = leads ? 31 - __clz(leads) : 0;
-      const int end = last ? __shfl_sync(0xffffffffu, lane - 1 + len, last) : 0;
+      const int end = __shfl_sync(0xffffffffu, lane - 1 + len, last);
       if (lane == 0) {
         nrun_s = __popc(leads);
-        ntab_s = max(n, end);
+        from_s = leads ? __ffs(leads) - 2 : 0;  // tokens that the runs span
+        to_s = leads ? end : 0;
       }
-    } else if (lane == 0) {
-      nrun_s = 0;
-      ntab_s = n;
     }
-  }
-  __syncthreads();
-  const int ntab = ntab_s;
-  for (int i = tid; i < ntab * p.half; i += kApThreads) {
-    const int64_t pos = p.positions[w0 + i / p.half];
-    const double f = p.inv_freq[i % p.half];
-    if constexpr (kF8) cs[i] = rope_cs64(pos, f, p.a);
-    else cs[i] = rope_cs(pos, f, (float)p.a);
   }
   __syncthreads();
 
   const bool inter = p.inter != 0;
-  // q rows
+  const LaneDims d = lane_dims(lane, p.half, inter);
   const T* qw = static_cast<const T*>(p.q_w);
   const T* kw = static_cast<const T*>(p.k_w);
-  for (int u = warp; u < n * p.hq; u += kApWarps) {
-    const int t = u / p.hq, h = u % p.hq;
-    const T* src = static_cast<const T*>(p.q) + (w0 + t) * p.q_stride + (int64_t)h * kApD;
-    float x[4];
-    norm_rotate<T>(*reinterpret_cast<const uint2*>(src + 4 * lane), qw, p.eps, cs + t * p.half,
-                   p.half, inter, lane, x);
-    T* dst = static_cast<T*>(p.q_out) + ((w0 + t) * p.hq + h) * kApD;
-    *reinterpret_cast<uint2*>(dst + 4 * lane) =
-        make_uint2(DT<T>::from_f2(x[0], x[1]), DT<T>::from_f2(x[2], x[3]));
+  if (kF8) {
+    const int from = from_s, to = to_s;
+    for (int i = tid; i < (to - from) * p.half; i += kApThreads)
+      cs64[from * p.half + i] = rope_cs64(p.positions[w0 + from + i / p.half],
+                                          p.inv_freq[i % p.half], p.a);
+  }
+
+  // q rows (and K rows of the dtype pool): kRows heads of a token a step
+  const int qb = (p.hq + kRows - 1) / kRows, kb = kF8 ? 0 : (p.hkv + kRows - 1) / kRows;
+  for (int u = warp; u < n * (qb + kb); u += kApWarps) {
+    const int t = u / (qb + kb), c = u % (qb + kb);
+    if (c < qb) {
+      const int h = c * kRows;
+      rows_f32<T, kRows>(static_cast<const T*>(p.q) + (w0 + t) * p.q_stride + (int64_t)h * kApD,
+                         static_cast<T*>(p.q_out) + ((w0 + t) * p.hq + h) * kApD,
+                         min(kRows, p.hq - h), qw, p.eps, cs + t * p.half, d, inter, lane);
+    } else {
+      const int h = (c - qb) * kRows;
+      const int64_t slot = slot_s[t + 1];
+      if (slot >= 0)
+        rows_f32<T, kRows>(static_cast<const T*>(p.k) + (w0 + t) * p.k_stride + (int64_t)h * kApD,
+                           static_cast<T*>(p.k_cache) + (slot * p.hkv + h) * kApD,
+                           min(kRows, p.hkv - h), kw, p.eps, cs + t * p.half, d, inter, lane);
+    }
   }
 
   if constexpr (!kF8) {
-    for (int u = warp; u < n * p.hkv * 2; u += kApWarps) {
-      const int kv = u & 1, t = (u >> 1) / p.hkv, h = (u >> 1) % p.hkv;
+    for (int u = warp; u < n * p.hkv; u += kApWarps) {
+      const int t = u / p.hkv, h = u % p.hkv;
       const int64_t slot = slot_s[t + 1];
       if (slot < 0) continue;
-      const T* src = kv ? static_cast<const T*>(p.v) + (w0 + t) * p.v_stride
-                        : static_cast<const T*>(p.k) + (w0 + t) * p.k_stride;
-      uint2 raw = *reinterpret_cast<const uint2*>(src + (int64_t)h * kApD + 4 * lane);
-      if (!kv) {
-        float x[4];
-        norm_rotate<T>(raw, kw, p.eps, cs + t * p.half, p.half, inter, lane, x);
-        raw = make_uint2(DT<T>::from_f2(x[0], x[1]), DT<T>::from_f2(x[2], x[3]));
-      }
-      T* dst = static_cast<T*>(kv ? p.v_cache : p.k_cache) + (slot * p.hkv + h) * kApD;
-      *reinterpret_cast<uint2*>(dst + 4 * lane) = raw;
+      const T* src = static_cast<const T*>(p.v) + (w0 + t) * p.v_stride + (int64_t)h * kApD;
+      T* dst = static_cast<T*>(p.v_cache) + (slot * p.hkv + h) * kApD;
+      *reinterpret_cast<uint2*>(dst + 4 * lane) = *reinterpret_cast<const uint2*>(src + 4 * lane);
     }
   } else {
-    for (int u = warp; u < nrun_s * p.hkv * 2; u += kApWarps) {
-      const int kv = u & 1, r = (u >> 1) / p.hkv, h = (u >> 1) % p.hkv;
+    __syncthreads();  // the f64 table
+    const int per = p.page / kApBlock, nk = nrun_s * p.hkv;
+    const int64_t row = (int64_t)p.hkv * kApD;
+    for (int u = warp; u < 2 * nk; u += kApWarps) {
+      const int kv = u >= nk, uu = kv ? u - nk : u;
+      const int r = uu / p.hkv, h = uu % p.hkv;
       const int t = lead_s[r], len = len_s[r];
-      const int64_t slot0 = slot_s[t + 1];
-      const int64_t blk = slot0 / kApBlock;
-      const int low = (int)(slot0 % kApBlock);
-      const int per = p.page / kApBlock;
+      const int64_t blk = slot_s[t + 1] / kApBlock;
+      const int low = (int)(slot_s[t + 1] % kApBlock);
       float* sp = p.scale + (((blk / per) * p.hkv + h) * per + blk % per) * 2 + kv;
       const float old = low ? *sp : 0.f;
-      const T* src = (kv ? static_cast<const T*>(p.v) + (w0 + t) * p.v_stride
-                         : static_cast<const T*>(p.k) + (w0 + t) * p.k_stride) +
-                     (int64_t)h * kApD + 4 * lane;
       const int64_t stride = kv ? p.v_stride : p.k_stride;
-      float x[kApBlock][4];
-      uint2 raw[kApBlock];
-#pragma unroll
-      for (int j = 0; j < kApBlock; ++j)
-        if (j < len) raw[j] = *reinterpret_cast<const uint2*>(src + j * stride);
+      const T* src = (kv ? static_cast<const T*>(p.v) : static_cast<const T*>(p.k)) +
+                     (w0 + t) * stride + (int64_t)h * kApD;
+      // V's rows are not rotated: four neighbouring dims a lane
+      const int da = kv ? 4 * lane : d.a, db = kv ? 4 * lane + 2 : d.b;
+      float x[2][8][4];
       float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < kApBlock; ++j) {
-        if (j < len) {
-          if (kv) {
-            const float2 a = DT<T>::to_f2(raw[j].x), b = DT<T>::to_f2(raw[j].y);
-            x[j][0] = a.x, x[j][1] = a.y, x[j][2] = b.x, x[j][3] = b.y;
-          } else {
-            R y[4];
-            norm_rotate<T>(raw[j], kw, p.eps, cs + (t + j) * p.half, p.half, inter, lane, y);
+      for (int g = 0; g < 2; ++g) {
+        if (8 * g < len) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[j][i] = f32_odd(y[i]);
+          for (int j = 0; j < 8; ++j) {
+            const T* s = src + (8 * g + j < len ? 8 * g + j : 0) * stride;
+            to_vals<T>(*reinterpret_cast<const uint32_t*>(s + da),
+                       *reinterpret_cast<const uint32_t*>(s + db), x[g][j]);
           }
+          if (!kv)
+            k_rows_f64<T>(x[g], len - 8 * g, kw, p.eps, cs64 + (t + 8 * g) * p.half, p.half, d,
+                          inter, lane);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float m = fabsf(x[j][i]);
-            amax = fmaxf(amax, m < INFINITY ? m : 0.f);
-          }
+          for (int j = 0; j < 8; ++j)
+            if (8 * g + j < len) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float m = fabsf(x[g][j][i]);
+                amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+              }
+            }
         }
       }
 #pragma unroll
@@ -275,18 +361,26 @@ __global__ void __launch_bounds__(kApThreads) rope_append_kernel(const AppendPar
       int e = block_exp(amax);
       if (low) e = max(e, e_old);
       const float inv = pow2i(-e);
-      uint8_t* cache = static_cast<uint8_t*>(kv ? p.v_cache : p.k_cache);
-      uint8_t* base = cache + (blk * kApBlock * p.hkv + h) * kApD + 4 * lane;
-      const int64_t row = (int64_t)p.hkv * kApD;
+      uint8_t* base = static_cast<uint8_t*>(kv ? p.v_cache : p.k_cache) +
+                      (blk * kApBlock * p.hkv + h) * kApD;
 #pragma unroll
-      for (int j = 0; j < kApBlock; ++j)
-        if (j < len)
-          *reinterpret_cast<uint32_t*>(base + (slot_s[t + 1 + j] % kApBlock) * row) =
-              e4m3x4(x[j][0] * inv, x[j][1] * inv, x[j][2] * inv, x[j][3] * inv);
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (8 * g + j < len) {
+            uint8_t* c = base + (slot_s[t + 1 + 8 * g + j] % kApBlock) * row;
+            const float* y = x[g][j];
+            const uint32_t w = e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+            *reinterpret_cast<uint16_t*>(c + da) = (uint16_t)w;
+            *reinterpret_cast<uint16_t*>(c + db) = (uint16_t)(w >> 16);
+          }
+        }
+      }
       if (e > e_old && low) {  // the kept rows move to the larger scale
         const float f = pow2i(max(e_old - e, -126));
+#pragma unroll 4
         for (int j = 0; j < low; ++j) {
-          uint32_t* c = reinterpret_cast<uint32_t*>(base + j * row);
+          uint32_t* c = reinterpret_cast<uint32_t*>(base + j * row + 4 * lane);
           float y[4];
           e4m3x4_f32(*c, y);
           *c = e4m3x4(y[0] * f, y[1] * f, y[2] * f, y[3] * f);
@@ -295,6 +389,14 @@ __global__ void __launch_bounds__(kApThreads) rope_append_kernel(const AppendPar
       if (lane == 0 && (!low || e > e_old)) *sp = pow2i(e);
     }
   }
+}
+
+template <typename T>
+int launch_append(const AppendParams& p, dim3 grid, size_t smem, cudaStream_t s) {
+  const bool f8 = p.scale != nullptr, wide = p.window > 1;
+  auto kern = f8 ? (wide ? rope_append_kernel<T, true, true> : rope_append_kernel<T, true, false>)
+                 : (wide ? rope_append_kernel<T, false, true> : rope_append_kernel<T, false, false>);
+  return launch_pdl(kern, grid, dim3(kApThreads), smem, s, "rope_append launch", p);
 }
 
 }  // namespace
@@ -372,17 +474,9 @@ extern "C" int nvkv_rope_append(const void* q, int64_t q_stride, const void* k, 
   p.window = (int)std::min<int64_t>(kApMaxWindow, std::max<int64_t>(1, num_tokens / (148 * 4)));
   const int64_t ctas = (num_tokens + p.window - 1) / p.window;
   if (ctas > 0x7fffffffLL) return set_error(NVKV_ERR_INVALID_ARG, "rope_append: too many tokens");
-  const int table = kv_scale ? p.window + kApBlock - 1 : p.window;
-  const size_t smem = (size_t)table * p.half * (kv_scale ? sizeof(double2) : sizeof(float2));
-  const dim3 grid((unsigned)ctas), block(kApThreads);
+  const size_t smem = (size_t)p.half * (p.window * sizeof(float2) +
+                                        (kv_scale ? (p.window + kApBlock - 1) * sizeof(double2) : 0));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == NVKV_DTYPE_BF16)
-    return kv_scale ? launch_pdl(rope_append_kernel<__nv_bfloat16, true>, grid, block, smem, s,
-                                 "rope_append launch", p)
-                    : launch_pdl(rope_append_kernel<__nv_bfloat16, false>, grid, block, smem, s,
-                                 "rope_append launch", p);
-  return kv_scale ? launch_pdl(rope_append_kernel<__half, true>, grid, block, smem, s,
-                               "rope_append launch", p)
-                  : launch_pdl(rope_append_kernel<__half, false>, grid, block, smem, s,
-                               "rope_append launch", p);
+  return dtype == NVKV_DTYPE_BF16 ? launch_append<__nv_bfloat16>(p, dim3((unsigned)ctas), smem, s)
+                                  : launch_append<__half>(p, dim3((unsigned)ctas), smem, s);
 }
