@@ -15,7 +15,7 @@
 // memory once for all heads, then each thread keeps one 16-byte unit of one
 // head (half layout: two 8-element vectors, r/2 apart; interleaved: one
 // vector of four pairs; a vector behind r: a copy) and walks the window's
-// tokens, four of them in flight.  Where r, the head size, a stride or an
+// tokens, two of them in flight.  Where r, the head size, a stride or an
 // address do not allow 16-byte vectors, a unit is a single pair.
 #include <math.h>
 
@@ -39,17 +39,29 @@ struct RopeParams {
   float a;
 };
 
-constexpr int kRopeFlight = 4;  // tokens in flight per thread
+// Tokens in flight per thread, and CTAs of one wave.  Measured at 16384 tokens,
+// 32 + 8 heads of 128 (51 us of traffic): 4 in flight (126 registers) 68.9 us, 2
+// in flight 61.0 / 57.7 / 63.5 / 58.8 us with 3 / 4 / 5 / 6 CTAs an SM.
+constexpr int kRopeFlight = 2;
+constexpr int kRopeThreads = 448;
+constexpr int kRopeWave = 148 * 4;
+constexpr int kRopeMaxWindow = 32;
 
 // VEC = 8: 16-byte units; 1: single pairs / elements.
 template <typename T, int VEC, bool kInter>
-__global__ void rope_kernel(const RopeParams p) {
-  extern __shared__ float2 cs[];  // [window][half]
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
+  // (cos, sin) of two pairs a float4: [window][VEC / 2 or 1][rotated units], so
+  // that neighbouring units read neighbouring words (8-byte entries for VEC = 1)
+  extern __shared__ __align__(16) float2 cs[];
+  constexpr int kPairs = VEC == 1 ? 1 : kInter ? 4 : 8;  // pairs of a unit
   const int64_t t0 = (int64_t)blockIdx.x * p.window;
   const int n = (int)min((int64_t)p.window, p.num_tokens - t0);
   const int nthr = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
-  for (int i = tid; i < n * p.half; i += nthr)
-    cs[i] = rope_cs(p.positions[t0 + i / p.half], p.inv_freq[i % p.half], p.a);
+  for (int i = tid; i < n * p.half; i += nthr) {
+    const int t = i / p.half, pr = i % p.half, u = pr / kPairs, w = pr % kPairs;
+    cs[t * p.half + (VEC == 1 ? pr : ((w >> 1) * p.rot_units + u) * 2 + (w & 1))] =
+        rope_cs(p.positions[t0 + t], p.inv_freq[pr], p.a);
+  }
   __syncthreads();
   using V = typename std::conditional<VEC == 8, uint4, uint16_t>::type;
   for (int u = threadIdx.x; u < p.units; u += blockDim.x) {
@@ -58,7 +70,6 @@ __global__ void rope_kernel(const RopeParams p) {
     const int e0 = rot ? (kInter && VEC == 1 ? 2 * u : u * VEC)
                        : 2 * p.half + (u - p.rot_units) * VEC;
     const int e1 = kInter ? e0 + 1 : e0 + p.half;
-    const int pair = kInter && VEC == 8 ? u * 4 : u * VEC;  // first pair of the unit
     for (int h = threadIdx.y; h < p.heads; h += blockDim.y) {
       const bool is_q = h < p.hq;
       const int64_t ho = (int64_t)(is_q ? h : h - p.hq) * p.d;
@@ -77,7 +88,7 @@ __global__ void rope_kernel(const RopeParams p) {
         for (int f = 0; f < kRopeFlight; ++f) {
           if (j + f >= n) break;
           if (rot) {
-            const float2* c = cs + (j + f) * p.half + pair;
+            const float2* c = cs + (j + f) * p.half + (VEC == 1 ? u : 2 * u);
             if constexpr (VEC == 1) {
               const float x0 = DT<T>::to_f(*reinterpret_cast<T*>(&a[f]));
               const float x1 = DT<T>::to_f(*reinterpret_cast<T*>(&b[f]));
@@ -90,15 +101,17 @@ __global__ void rope_kernel(const RopeParams p) {
               uint32_t* wb = reinterpret_cast<uint32_t*>(&b[f]);
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
+                // pairs 2w, 2w + 1 of the unit (interleaved: pair w, half of an entry)
+                const float4 r = *reinterpret_cast<const float4*>(
+                    c + (kInter ? w >> 1 : w) * 2 * p.rot_units);
                 if (kInter) {
                   const float2 x = DT<T>::to_f2(wa[w]);
-                  const float2 r = c[w];
-                  wa[w] = DT<T>::from_f2(x.x * r.x - x.y * r.y, x.y * r.x + x.x * r.y);
+                  const float cc = w & 1 ? r.z : r.x, ss = w & 1 ? r.w : r.y;
+                  wa[w] = DT<T>::from_f2(x.x * cc - x.y * ss, x.y * cc + x.x * ss);
                 } else {
                   const float2 x = DT<T>::to_f2(wa[w]), y = DT<T>::to_f2(wb[w]);
-                  const float2 r0 = c[2 * w], r1 = c[2 * w + 1];
-                  wa[w] = DT<T>::from_f2(x.x * r0.x - y.x * r0.y, x.y * r1.x - y.y * r1.y);
-                  wb[w] = DT<T>::from_f2(y.x * r0.x + x.x * r0.y, y.y * r1.x + x.y * r1.y);
+                  wa[w] = DT<T>::from_f2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w);
+                  wb[w] = DT<T>::from_f2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w);
                 }
               }
             }
@@ -260,11 +273,13 @@ extern "C" int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t
   p.rot_units = vec ? rot_dim / (inter ? 8 : 16) : rot_dim / 2;
   const int copies = in_place ? 0 : (head_dim - rot_dim) / (vec ? 8 : 1);
   p.units = p.rot_units + copies;
-  // ~6 CTAs an SM before windows grow; a window's table is shared by all heads
-  p.window = (int)std::min<int64_t>(8, std::max<int64_t>(1, num_tokens / (148 * 6)));
+  // One wave of CTAs: a CTA costs two dependent loads, the table and a barrier
+  // before it streams (the same 16384 tokens with four in flight: windows of 1 / 2
+  // / 4 / 8 tokens 237 / 140 / 93 / 75 us).
+  p.window = (int)std::min<int64_t>(kRopeMaxWindow, (num_tokens + kRopeWave - 1) / kRopeWave);
   const int bx = std::min(p.units, 64);
-  const int rounds = std::max(1, (p.heads * bx + 383) / 384);
-  const int by = std::max(1, std::min((p.heads + rounds - 1) / rounds, 1024 / bx));
+  const int rounds = (p.heads * bx + 383) / 384;
+  const int by = (p.heads + rounds - 1) / rounds;  // bx * by < 384 + bx
   const int64_t ctas = (num_tokens + p.window - 1) / p.window;
   if (ctas > 0x7fffffffLL) return set_error(NVKV_ERR_INVALID_ARG, "rope: too many tokens");
   const size_t smem = (size_t)p.window * p.half * sizeof(float2);

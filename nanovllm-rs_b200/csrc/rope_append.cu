@@ -7,13 +7,13 @@
 // code = e4m3(x 2^-e); rows that the block already held move by code' =
 // e4m3(code 2^(e_kept - e)).  K is normalised and rotated in f64 and reaches
 // e4m3 by ONE rounding (to f32 by rounding to odd, which the conversion to four
-// significant bits cannot tell from the exact value), so the codes are a
-// function of the formulas and not of the f32 arithmetic's order, and tests
-// compare them bit by bit.  q and the dtype pool use f32 and round once.
+// significant bits cannot tell from the f64 value), so the codes are a function of
+// the formulas and not of the f32 arithmetic's order, and tests compare them bit
+// by bit.  q and the dtype pool use f32 and round once.
 //
 // Layout.  A CTA of 8 warps owns a window of W tokens: the cos / sin of those
-// tokens go to shared memory once (f32 for q; f64 for the tokens of the runs,
-// up to 15 of them past the window); then warps take q rows and K / V units,
+// tokens (and of the up to 15 that follow in the last run) go to shared memory
+// once; then warps take q rows and K / V units,
 // every pair in one lane.  A unit is one run (the call's tokens of one block),
 // one kv head, K or V: the warp holds all of its up to 16 rows in registers (64
 // values a lane), so the maximum, the scale and the codes come from one read.
@@ -34,7 +34,6 @@ constexpr int kApWarps = kApThreads / 32;
 constexpr int kApMaxWindow = 16;
 constexpr int kApTable = kApMaxWindow + kApBlock - 1;  // tokens a table can hold
 constexpr int kApMinE = -100;
-
 struct AppendParams {
   const void *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;
@@ -54,10 +53,11 @@ struct AppendParams {
   int* err;
 };
 
-// f64 -> f32 rounded to odd: toward zero, the last bit set if anything was cut.
+// f64 -> f32 rounded to odd: toward zero, the last bit set if anything was cut
+// (the low 29 bits, in f32's normal range; below it every code is 0 either way).
 __device__ __forceinline__ float f32_odd(double x) {
-  const float f = __double2float_rz(x);
-  return (double)f == x || x != x ? f : __uint_as_float(__float_as_uint(f) | 1u);
+  const uint32_t cut = (uint32_t)__double2loint(x) & 0x1fffffffu;
+  return __uint_as_float(__float_as_uint(__double2float_rz(x)) | (cut ? 1u : 0u));
 }
 
 // least e >= -100 with amax <= 448 * 2^e = 1.75 * 2^(e + 8)
@@ -83,50 +83,68 @@ __device__ __forceinline__ void e4m3x4_f32(uint32_t w, float* f) {
   f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
 }
 
-// A lane's dims of a rotated row: the chunks x[a], x[a + 1] and x[b], x[b + 1],
-// chosen so that every pair sits in one lane: pairs 2 lane and 2 lane + 1 of
-// either layout while lane < half / 2, dims that pass through behind them.
+// Packed two-lane f32 arithmetic (sm_100): one instruction for two values.
+__device__ __forceinline__ uint64_t pk(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpk(uint64_t r) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// Half a warp takes a head row, 8 dims a lane in two chunks of four: x[a ..
+// a + 3] and x[b .. b + 3].  While sub = lane % 16 < half / 4 they are pairs
+// 4 sub .. 4 sub + 3 of either layout; the lanes behind pass their dims through.
 struct LaneDims {
   int a, b;
   bool rot;
 };
-__device__ __forceinline__ LaneDims lane_dims(int lane, int half, bool inter) {
+template <bool kInter>
+__device__ __forceinline__ LaneDims lane_dims(int sub, int half) {
   LaneDims d;
-  d.rot = lane < half / 2;
-  d.a = d.rot && !inter ? 2 * lane : 4 * lane;  // half: pass-through dims 4 lane .. are >= 2 half
-  d.b = d.rot && !inter ? half + 2 * lane : 4 * lane + 2;
+  d.rot = sub < half / 4;
+  d.a = d.rot && !kInter ? 4 * sub : 8 * sub;  // (8 sub >= 2 half behind the rotated part)
+  d.b = d.rot && !kInter ? half + 4 * sub : 8 * sub + 4;
   return d;
 }
 
-template <typename T, typename R>
-__device__ __forceinline__ void to_vals(uint32_t a, uint32_t b, R (&x)[4]) {
-  const float2 u = DT<T>::to_f2(a), v = DT<T>::to_f2(b);
-  x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
+// The eight values as pair partners: X = first members, Y = second ones, of
+// pairs 4 sub .. 4 sub + 3 (for lanes that pass through: any fixed order).
+template <typename T, bool kInter, typename R>
+__device__ __forceinline__ void to_pairs(const uint2 wa, const uint2 wb, R (&x)[4], R (&y)[4]) {
+  const float2 a0 = DT<T>::to_f2(wa.x), a1 = DT<T>::to_f2(wa.y);
+  const float2 b0 = DT<T>::to_f2(wb.x), b1 = DT<T>::to_f2(wb.y);
+  if (kInter) {
+    x[0] = a0.x, y[0] = a0.y, x[1] = a1.x, y[1] = a1.y;
+    x[2] = b0.x, y[2] = b0.y, x[3] = b1.x, y[3] = b1.y;
+  } else {
+    x[0] = a0.x, x[1] = a0.y, x[2] = a1.x, x[3] = a1.y;
+    y[0] = b0.x, y[1] = b0.y, y[2] = b1.x, y[3] = b1.y;
+  }
 }
 
-// x rotated by the lane's two pairs' (cos, sin)
-template <typename R, typename C>
-__device__ __forceinline__ void rotate(R (&x)[4], const C c0, const C c1, bool inter) {
-  const R p = x[0], q = inter ? x[1] : x[2], r = inter ? x[2] : x[1], s = x[3];
-  const R y0 = p * c0.x - q * c0.y, y1 = q * c0.x + p * c0.y;
-  const R y2 = r * c1.x - s * c1.y, y3 = s * c1.x + r * c1.y;
-  x[0] = y0;
-  x[1] = inter ? y1 : y2;
-  x[2] = inter ? y2 : y1;
-  x[3] = y3;
-}
-
-// Sums over the warp of N values a lane (N = 4 or 8): halving exchanges leave
-// row j's sum in the lanes with j in their upper bits (9 shuffles for 8 rows
-// instead of 40); row_lane(j) is one of them.
+// Sums over half a warp of N values a lane: halving exchanges leave value j's
+// sum in the lanes whose upper bits spell j (8 shuffles for 8 values, not 32).
 template <int N>
-__device__ __forceinline__ int row_lane(int j) {
-  return N == 8 ? ((j >> 2) & 1) << 4 | ((j >> 1) & 1) << 3 | (j & 1) << 2
-                : ((j >> 1) & 1) << 4 | (j & 1) << 3;
+__device__ __forceinline__ int sum_lane(int j, int lane) {
+  return (lane & 16) | j * (16 / N);
 }
 template <int N, typename R>
-__device__ __forceinline__ R row_sums(R (&v)[N], int lane) {
-  int m = 16;
+__device__ __forceinline__ R half_sums(R (&v)[N], int lane) {
+  int m = 8;
 #pragma unroll
   for (int n = N; n > 1; n >>= 1, m >>= 1) {
     const bool up = lane & m;
@@ -141,101 +159,330 @@ __device__ __forceinline__ R row_sums(R (&v)[N], int lane) {
   return v[0];
 }
 
-// Up to N head rows (128 apart) of one token: norm, rotation, one rounding.
-template <typename T, int N>
-__device__ __forceinline__ void rows_f32(const T* src, T* dst, int n, const T* w, float eps,
-                                         const float2* cs, const LaneDims d, bool inter, int lane) {
-  uint32_t ra[N], rb[N];
+// A token's rotation with the norm's weights folded in, for the lane's four
+// pairs: y0 = inv (x0 A - x1 B), y1 = inv (x1 C + x0 E); packed by two pairs.
+struct Coef {
+  uint64_t a[2], b[2], c[2], e[2];
+};
+template <typename T, bool kInter>
+__device__ __forceinline__ Coef token_coef(const float2* cs, const T* w, const LaneDims d, int sub) {
+  float wx[4] = {1.f, 1.f, 1.f, 1.f}, wy[4] = {1.f, 1.f, 1.f, 1.f};
+  if (w)
+    to_pairs<T, kInter>(*reinterpret_cast<const uint2*>(w + d.a),
+                        *reinterpret_cast<const uint2*>(w + d.b), wx, wy);
+  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (d.rot) {
+    const float4 p0 = *reinterpret_cast<const float4*>(cs + 4 * sub);
+    const float4 p1 = *reinterpret_cast<const float4*>(cs + 4 * sub + 2);
+    c[0] = p0.x, s[0] = p0.y, c[1] = p0.z, s[1] = p0.w;
+    c[2] = p1.x, s[2] = p1.y, c[3] = p1.z, s[3] = p1.w;
+  }
+  Coef f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f.a[i] = pk(wx[2 * i] * c[2 * i], wx[2 * i + 1] * c[2 * i + 1]);
+    f.b[i] = pk(-wy[2 * i] * s[2 * i], -wy[2 * i + 1] * s[2 * i + 1]);
+    f.c[i] = pk(wy[2 * i] * c[2 * i], wy[2 * i + 1] * c[2 * i + 1]);
+    f.e[i] = pk(wx[2 * i] * s[2 * i], wx[2 * i + 1] * s[2 * i + 1]);
+  }
+  return f;
+}
+
+// Up to 2 N head rows (128 apart) of one token: norm, rotation, one rounding.
+template <typename T, int N, bool kInter>
+__device__ __forceinline__ void rows_f32(const T* src, T* dst, int n, bool norm, float eps,
+                                         const Coef& f, const LaneDims d, int lane) {
+  const int grp = lane >> 4;
+  float x[N][4], y[N][4];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const T* s = src + (j < n ? j : 0) * kApD;
-    ra[j] = *reinterpret_cast<const uint32_t*>(s + d.a);
-    rb[j] = *reinterpret_cast<const uint32_t*>(s + d.b);
+    const T* s = src + (2 * j + grp < n ? 2 * j + grp : 0) * kApD;
+    to_pairs<T, kInter>(*reinterpret_cast<const uint2*>(s + d.a),
+                        *reinterpret_cast<const uint2*>(s + d.b), x[j], y[j]);
   }
-  const float2 c0 = d.rot ? cs[2 * lane] : make_float2(1.f, 0.f);
-  const float2 c1 = d.rot ? cs[2 * lane + 1] : make_float2(1.f, 0.f);
-  float inv = 1.f, wv[4] = {1.f, 1.f, 1.f, 1.f};
-  if (w) {
-    to_vals<T>(*reinterpret_cast<const uint32_t*>(w + d.a),
-               *reinterpret_cast<const uint32_t*>(w + d.b), wv);
+  float inv = 1.f;
+  if (norm) {
     float ss[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      float x[4];
-      to_vals<T>(ra[j], rb[j], x);
-      ss[j] = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+      uint64_t q = mul2(pk(x[j][0], x[j][1]), pk(x[j][0], x[j][1]));
+      q = fma2(pk(x[j][2], x[j][3]), pk(x[j][2], x[j][3]), q);
+      q = fma2(pk(y[j][0], y[j][1]), pk(y[j][0], y[j][1]), q);
+      q = fma2(pk(y[j][2], y[j][3]), pk(y[j][2], y[j][3]), q);
+      ss[j] = unpk(q).x + unpk(q).y;
     }
-    inv = 1.f / sqrtf(row_sums<N>(ss, lane) * (1.f / kApD) + eps);
+    inv = 1.f / sqrtf(half_sums<N>(ss, lane) * (1.f / kApD) + eps);
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    float x[4];
-    to_vals<T>(ra[j], rb[j], x);
-    if (w) {
-      const float f = __shfl_sync(0xffffffffu, inv, row_lane<N>(j));
+    const float g = norm ? __shfl_sync(0xffffffffu, inv, sum_lane<N>(j, lane)) : 1.f;
+    const uint64_t g2 = pk(g, g);
+    float2 ox[2], oy[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = x[i] * f * wv[i];
-    }
-    if (d.rot) rotate(x, c0, c1, inter);
-    if (j < n) {
-      *reinterpret_cast<uint32_t*>(dst + j * kApD + d.a) = DT<T>::from_f2(x[0], x[1]);
-      *reinterpret_cast<uint32_t*>(dst + j * kApD + d.b) = DT<T>::from_f2(x[2], x[3]);
-    }
-  }
-}
-
-// K rows j0 .. j0 + 7 of a run in f64: x[j] becomes the normalised, rotated
-// value rounded to odd.
-template <typename T>
-__device__ __forceinline__ void k_rows_f64(float (&x)[8][4], int n, const T* w, float eps,
-                                           const double2* cs, int half, const LaneDims d,
-                                           bool inter, int lane) {
-  double inv = 1.0, wv[4];
-  if (w) {
-    to_vals<T>(*reinterpret_cast<const uint32_t*>(w + d.a),
-               *reinterpret_cast<const uint32_t*>(w + d.b), wv);
-    double ss[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ss[j] = 0.0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss[j] = fma((double)x[j][i], (double)x[j][i], ss[j]);
-    }
-    inv = rsqrt(row_sums<8>(ss, lane) * (1.0 / kApD) + (double)eps);  // for this lane's row
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (j < n) {
-      double y[4] = {x[j][0], x[j][1], x[j][2], x[j][3]};
-      if (w) {
-        const double f = __shfl_sync(0xffffffffu, inv, row_lane<8>(j));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = y[i] * f * wv[i];
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t X = pk(x[j][2 * i], x[j][2 * i + 1]), Y = pk(y[j][2 * i], y[j][2 * i + 1]);
+      uint64_t u = mul2(X, f.a[i]), v = mul2(Y, f.c[i]);
+      if (d.rot) {
+        u = fma2(Y, f.b[i], u);
+        v = fma2(X, f.e[i], v);
       }
-      if (d.rot) rotate(y, cs[j * half + 2 * lane], cs[j * half + 2 * lane + 1], inter);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[j][i] = f32_odd(y[i]);
+      if (norm) {
+        u = mul2(u, g2);
+        v = mul2(v, g2);
+      }
+      ox[i] = unpk(u);
+      oy[i] = unpk(v);
+    }
+    if (2 * j + grp < n) {
+      T* t = dst + (2 * j + grp) * kApD;
+      uint2 wa, wb;
+      if (kInter) {
+        wa = make_uint2(DT<T>::from_f2(ox[0].x, oy[0].x), DT<T>::from_f2(ox[0].y, oy[0].y));
+        wb = make_uint2(DT<T>::from_f2(ox[1].x, oy[1].x), DT<T>::from_f2(ox[1].y, oy[1].y));
+      } else {
+        wa = make_uint2(DT<T>::from_f2(ox[0].x, ox[0].y), DT<T>::from_f2(ox[1].x, ox[1].y));
+        wb = make_uint2(DT<T>::from_f2(oy[0].x, oy[0].y), DT<T>::from_f2(oy[1].x, oy[1].y));
+      }
+      *reinterpret_cast<uint2*>(t + d.a) = wa;
+      *reinterpret_cast<uint2*>(t + d.b) = wb;
     }
   }
 }
 
-// kWide: windows of several tokens (8 rows in flight a warp); else a decode
-// step's single tokens (4, so that eight warps share 32 heads).
-template <typename T, bool kF8, bool kWide>
-__global__ void __launch_bounds__(kApThreads, 2) rope_append_kernel(const AppendParams p) {
-  constexpr int kRows = kWide ? 8 : 4;
+// A barrier of warps 2 i and 2 i + 1.
+__device__ __forceinline__ void pair_barrier(int warp) {
+  asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+}
+
+// One run of one kv head.  Of a warp's rows, row 2 j + lane / 16 sits in x[j] /
+// y[j] (values as pairs for K, eight neighbouring dims for V); rows past the run
+// repeat its row 0 and are not stored.
+struct Unit {
+  uint8_t* base;  // the block's row 0, this head
+  float* scale;
+  const int64_t* slot;  // shared: the run's slots
+  int len, low, row0;
+  int64_t row;  // bytes between rows
+};
+
+// The warp's largest finite |value|.
+template <int N>
+__device__ __forceinline__ float warp_amax(const float (&x)[N][4], const float (&y)[N][4]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m = max(m, max(__float_as_uint(x[j][i]) & 0x7fffffffu, __float_as_uint(y[j][i]) & 0x7fffffffu));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (m >= 0x7f800000u) {  // an infinity or NaN among them: leave those out
+    m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = __float_as_uint(x[j][i]) & 0x7fffffffu;
+        const uint32_t b = __float_as_uint(y[j][i]) & 0x7fffffffu;
+        m = max(m, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
+      }
+    m = __reduce_max_sync(0xffffffffu, m);
+  }
+  return __uint_as_float(m);
+}
+
+// Codes of a warp's rows once the block's largest value is known; the warp of row
+// 0 also moves kept rows and writes the scale.  kFull: a whole block, 16 rows.
+template <int N, bool kFull>
+__device__ __forceinline__ void encode_rows(const float (&x)[N][4], const float (&y)[N][4],
+                                            const Unit& u, float old, float amax, int da, int db,
+                                            bool inter, int lane) {
+  const int grp = lane >> 4;
+  const int e_old = max(kApMinE, (int)(__float_as_uint(old) >> 23 & 0xffu) - 127);
+  int e = block_exp(amax);
+  if (!kFull && u.low) e = max(e, e_old);
+  const float inv = pow2i(-e);
+  uint8_t* c = u.base + (kFull ? (u.row0 + grp) * u.row : 0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int r = u.row0 + 2 * j + grp;
+    uint32_t wa, wb;
+    if (inter) {
+      wa = e4m3x4(x[j][0] * inv, y[j][0] * inv, x[j][1] * inv, y[j][1] * inv);
+      wb = e4m3x4(x[j][2] * inv, y[j][2] * inv, x[j][3] * inv, y[j][3] * inv);
+    } else {
+      wa = e4m3x4(x[j][0] * inv, x[j][1] * inv, x[j][2] * inv, x[j][3] * inv);
+      wb = e4m3x4(y[j][0] * inv, y[j][1] * inv, y[j][2] * inv, y[j][3] * inv);
+    }
+    if (kFull || r < u.len) {
+      if (!kFull) c = u.base + (u.slot[r] % kApBlock) * u.row;
+      *reinterpret_cast<uint32_t*>(c + da) = wa;
+      *reinterpret_cast<uint32_t*>(c + db) = wb;
+    }
+    if (kFull) c += 2 * u.row;
+  }
+  if (u.row0 == 0) {
+    if (!kFull && e > e_old && u.low) {
+      const float f = pow2i(max(e_old - e, -126));
+#pragma unroll 4
+      for (int j = 0; j < u.low; ++j) {
+        uint32_t* k = reinterpret_cast<uint32_t*>(u.base + j * u.row + 4 * lane);
+        float v[4];
+        e4m3x4_f32(*k, v);
+        *k = e4m3x4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+      }
+    }
+    if (lane == 0 && (kFull || !u.low || e > e_old)) *u.scale = pow2i(e);
+  }
+}
+
+// A warp's rows of a run as pairs (x, y); rows past it repeat its row 0, row
+// pairs past it are zero and count for nothing in the maximum.
+template <typename T, int N, bool kFull, bool kInter>
+__device__ __forceinline__ void load_rows(float (&x)[N][4], float (&y)[N][4], const T* src,
+                                          int64_t stride, const Unit& u, int pairs, int da, int db,
+                                          int grp) {
+  const T* s = src + (kFull ? (u.row0 + grp) * stride : 0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (kFull || j < pairs) {
+      if (!kFull) {
+        const int r = u.row0 + 2 * j + grp;
+        s = src + (r < u.len ? r : 0) * stride;
+      }
+      to_pairs<T, kInter>(*reinterpret_cast<const uint2*>(s + da),
+                          *reinterpret_cast<const uint2*>(s + db), x[j], y[j]);
+      if (kFull) s += 2 * stride;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[j][c] = y[j][c] = 0.f;
+    }
+  }
+}
+
+// K rows in f64: norm, rotation, rounding to odd.  cs: the f64 table at the run's
+// first token.
+template <typename T, int N, bool kFull, bool kInter>
+__device__ __forceinline__ void k_rows(float (&x)[N][4], float (&y)[N][4], const Unit& u,
+                                       int pairs, const T* w, float eps, const double2* cs,
+                                       int half, const LaneDims d, int lane) {
+  const int sub = lane & 15, grp = lane >> 4;
+  double inv = 1.0;
+  float wx[4] = {1.f, 1.f, 1.f, 1.f}, wy[4] = {1.f, 1.f, 1.f, 1.f};
+  if (w) {
+    to_pairs<T, kInter>(*reinterpret_cast<const uint2*>(w + d.a),
+                        *reinterpret_cast<const uint2*>(w + d.b), wx, wy);
+    double ss[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      ss[j] = 0.0;
+      if (kFull || j < pairs) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          ss[j] = fma((double)x[j][c], (double)x[j][c], ss[j]);
+          ss[j] = fma((double)y[j][c], (double)y[j][c], ss[j]);
+        }
+      }
+    }
+    inv = rsqrt(half_sums<N>(ss, lane) * (1.0 / kApD) + (double)eps);
+  }
+  const double2* c64 = cs + (kFull ? (u.row0 + grp) * half : 0) + sub;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (kFull || j < pairs) {
+      const double g = w ? __shfl_sync(0xffffffffu, inv, sum_lane<N>(j, lane)) : 1.0;
+      if (!kFull) {
+        const int r = u.row0 + 2 * j + grp;
+        c64 = cs + (r < u.len ? r : 0) * half + sub;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        double a = x[j][c], b = y[j][c];
+        if (w) {
+          a *= (double)wx[c];
+          b *= (double)wy[c];
+        }
+        if (d.rot) {
+          const double2 k = c64[c * (half / 4)];
+          const double a1 = a * k.x - b * k.y;
+          b = b * k.x + a * k.y;
+          a = a1;
+        }
+        x[j][c] = f32_odd(a * g);
+        y[j][c] = f32_odd(b * g);
+      }
+    }
+    if (kFull) c64 += 2 * half;
+  }
+}
+
+// One unit: a run and kv head, K and (kWide) V.
+template <typename T, int N, bool kWide, bool kFull, bool kInter>
+__device__ __forceinline__ void unit(const AppendParams& p, Unit u, const T* ks, const T* vs,
+                                     float* scale, int64_t block0, bool only_v, const double2* cs,
+                                     const LaneDims d, float (*duo)[2], int warp, int lane) {
+  const int sub = lane & 15, grp = lane >> 4, va = 8 * sub;  // V: eight neighbouring dims a lane
+  const int pairs = max(1, (u.len - u.row0 + 1) / 2);        // row pairs in use
+  float x[N][4], y[N][4], old_k = 0.f, old_v = 0.f;
+  if (!kFull && u.low) old_k = scale[0], old_v = scale[1];
+  if (only_v) {
+    load_rows<T, N, kFull, false>(x, y, vs, p.v_stride, u, pairs, va, va + 4, grp);
+  } else {
+    load_rows<T, N, kFull, kInter>(x, y, ks, p.k_stride, u, pairs, d.a, d.b, grp);
+    k_rows<T, N, kFull, kInter>(x, y, u, pairs, static_cast<const T*>(p.k_w), p.eps, cs, p.half, d,
+                                lane);
+  }
+  float amax = warp_amax(x, y);
+  if (kWide) {  // the other warp's; its scale has been read by the first barrier
+    if (lane == 0) duo[warp][0] = amax;
+    pair_barrier(warp);
+    amax = fmaxf(amax, duo[warp ^ 1][0]);
+  }
+  u.base = static_cast<uint8_t*>(only_v ? p.v_cache : p.k_cache) + block0;
+  u.scale = scale + (only_v ? 1 : 0);
+  encode_rows<N, kFull>(x, y, u, only_v ? old_v : old_k, amax, only_v ? va : d.a,
+                        only_v ? va + 4 : d.b, kInter && !only_v, lane);
+  if (kWide) {
+    load_rows<T, N, kFull, false>(x, y, vs, p.v_stride, u, pairs, va, va + 4, grp);
+    float vmax = warp_amax(x, y);
+    if (lane == 0) duo[warp][1] = vmax;
+    pair_barrier(warp);
+    vmax = fmaxf(vmax, duo[warp ^ 1][1]);
+    u.base = static_cast<uint8_t*>(p.v_cache) + block0;
+    u.scale = scale + 1;
+    encode_rows<N, kFull>(x, y, u, old_v, vmax, va, va + 4, false, lane);
+  }
+}
+
+// kWide: windows of several tokens (8 rows in flight a warp, two warps a run:
+// registers for three CTAs an SM); else a decode step's single tokens (4 rows in
+// flight, so that eight warps share 32 heads, and a warp a run, mostly one row).
+template <typename T, bool kF8, bool kWide, bool kInter>
+__global__ void __launch_bounds__(kApThreads, kWide ? 3 : 2)
+    rope_append_kernel(const AppendParams p) {
+  constexpr int kN = kWide ? 4 : 2, kRows = 2 * kN;
+  constexpr int kM = kWide ? 4 : 8;  // row pairs of a warp's part of a run
   extern __shared__ __align__(16) uint8_t smem[];
-  double2* cs64 = reinterpret_cast<double2*>(smem);  // [run tokens][half], fp8b pool
+  // f64 (cos, sin) of the run tokens, [token][pair % 4][pair / 4]: lanes read
+  // neighbouring entries; then f32 ones, [token][half]
+  double2* cs64 = reinterpret_cast<double2*>(smem);
   float2* cs = reinterpret_cast<float2*>(
       smem + (kF8 ? (size_t)(p.window + kApBlock - 1) * p.half * sizeof(double2) : 0));
   __shared__ int64_t slot_s[kApTable + 1];  // slots of tokens w0 - 1 ..
   __shared__ int lead_s[kApMaxWindow], len_s[kApMaxWindow], nrun_s, from_s, to_s;
+  __shared__ float duo_s[kApWarps][2];
   const int64_t w0 = (int64_t)blockIdx.x * p.window;
   const int n = (int)min((int64_t)p.window, p.num_tokens - w0);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane & 15;
+  const LaneDims d = lane_dims<kInter>(sub, p.half);
+  const T* qw = static_cast<const T*>(p.q_w);
+  const T* kw = static_cast<const T*>(p.k_w);
   pdl_wait();  // nothing is read or written before: the launch may overlap the kernel before it
-  for (int i = tid; i < n * p.half; i += kApThreads)
-    cs[i] = rope_cs(p.positions[w0 + i / p.half], p.inv_freq[i % p.half], (float)p.a);
+  // tables: a thread keeps one pair, 4 tokens a step
+  const int pr = tid % 64;
+  const double fr = pr < p.half ? p.inv_freq[pr] : 0.0;
+  if (pr < p.half)
+    for (int t = tid / 64; t < n; t += kApThreads / 64)
+      cs[t * p.half + pr] = rope_cs(p.positions[w0 + t], fr, (float)p.a);
   if (warp == kApWarps - 1) {
     const int64_t t = w0 - 1 + lane;  // lane 0: the token before the window
     int64_t s = -1;
@@ -273,130 +520,84 @@ __global__ void __launch_bounds__(kApThreads, 2) rope_append_kernel(const Append
     }
   }
   __syncthreads();
+  if (kF8 && pr < p.half)
+    for (int t = from_s + tid / 64; t < to_s; t += kApThreads / 64)
+      cs64[t * p.half + (pr & 3) * (p.half / 4) + (pr >> 2)] =
+          rope_cs64(p.positions[w0 + t], fr, p.a);
 
-  const bool inter = p.inter != 0;
-  const LaneDims d = lane_dims(lane, p.half, inter);
-  const T* qw = static_cast<const T*>(p.q_w);
-  const T* kw = static_cast<const T*>(p.k_w);
-  if (kF8) {
-    const int from = from_s, to = to_s;
-    for (int i = tid; i < (to - from) * p.half; i += kApThreads)
-      cs64[from * p.half + i] = rope_cs64(p.positions[w0 + from + i / p.half],
-                                          p.inv_freq[i % p.half], p.a);
-  }
-
-  // q rows (and K rows of the dtype pool): kRows heads of a token a step
-  const int qb = (p.hq + kRows - 1) / kRows, kb = kF8 ? 0 : (p.hkv + kRows - 1) / kRows;
-  for (int u = warp; u < n * (qb + kb); u += kApWarps) {
-    const int t = u / (qb + kb), c = u % (qb + kb);
-    if (c < qb) {
-      const int h = c * kRows;
-      rows_f32<T, kRows>(static_cast<const T*>(p.q) + (w0 + t) * p.q_stride + (int64_t)h * kApD,
-                         static_cast<T*>(p.q_out) + ((w0 + t) * p.hq + h) * kApD,
-                         min(kRows, p.hq - h), qw, p.eps, cs + t * p.half, d, inter, lane);
-    } else {
-      const int h = (c - qb) * kRows;
-      const int64_t slot = slot_s[t + 1];
-      if (slot >= 0)
-        rows_f32<T, kRows>(static_cast<const T*>(p.k) + (w0 + t) * p.k_stride + (int64_t)h * kApD,
-                           static_cast<T*>(p.k_cache) + (slot * p.hkv + h) * kApD,
-                           min(kRows, p.hkv - h), kw, p.eps, cs + t * p.half, d, inter, lane);
+  // rows of single tokens: a warp per token when the window is wide, else a few
+  // heads of the token
+  const int parts = kWide ? 1 : kApWarps, part = kWide ? 0 : warp;
+  {
+    for (int t = kWide ? warp : 0; t < n; t += kWide ? kApWarps : 1) {
+      const int64_t tok = w0 + t;
+      const Coef f = token_coef<T, kInter>(cs + t * p.half, qw, d, sub);
+      for (int h = part * kRows; h < p.hq; h += parts * kRows)
+        rows_f32<T, kN, kInter>(static_cast<const T*>(p.q) + tok * p.q_stride + (int64_t)h * kApD,
+                                static_cast<T*>(p.q_out) + (tok * p.hq + h) * kApD,
+                                min(kRows, p.hq - h), qw != nullptr, p.eps, f, d, lane);
     }
   }
-
   if constexpr (!kF8) {
-    for (int u = warp; u < n * p.hkv; u += kApWarps) {
-      const int t = u / p.hkv, h = u % p.hkv;
-      const int64_t slot = slot_s[t + 1];
+    for (int t = kWide ? warp : 0; t < n; t += kWide ? kApWarps : 1) {
+      const int64_t tok = w0 + t, slot = slot_s[t + 1];
       if (slot < 0) continue;
-      const T* src = static_cast<const T*>(p.v) + (w0 + t) * p.v_stride + (int64_t)h * kApD;
-      T* dst = static_cast<T*>(p.v_cache) + (slot * p.hkv + h) * kApD;
-      *reinterpret_cast<uint2*>(dst + 4 * lane) = *reinterpret_cast<const uint2*>(src + 4 * lane);
+      const Coef f = token_coef<T, kInter>(cs + t * p.half, kw, d, sub);
+      for (int h = part * kRows; h < p.hkv; h += parts * kRows)
+        rows_f32<T, kN, kInter>(static_cast<const T*>(p.k) + tok * p.k_stride + (int64_t)h * kApD,
+                                static_cast<T*>(p.k_cache) + (slot * p.hkv + h) * kApD,
+                                min(kRows, p.hkv - h), kw != nullptr, p.eps, f, d, lane);
+      const T* src = static_cast<const T*>(p.v) + tok * p.v_stride;
+      T* dst = static_cast<T*>(p.v_cache) + slot * p.hkv * kApD;
+#pragma unroll 4
+      for (int c = part * 32 + lane; c < p.hkv * 32; c += parts * 32)
+        *reinterpret_cast<uint2*>(dst + 4 * c) = *reinterpret_cast<const uint2*>(src + 4 * c);
     }
   } else {
     __syncthreads();  // the f64 table
-    const int per = p.page / kApBlock, nk = nrun_s * p.hkv;
-    const int64_t row = (int64_t)p.hkv * kApD;
-    for (int u = warp; u < 2 * nk; u += kApWarps) {
-      const int kv = u >= nk, uu = kv ? u - nk : u;
-      const int r = uu / p.hkv, h = uu % p.hkv;
-      const int t = lead_s[r], len = len_s[r];
-      const int64_t blk = slot_s[t + 1] / kApBlock;
-      const int low = (int)(slot_s[t + 1] % kApBlock);
-      float* sp = p.scale + (((blk / per) * p.hkv + h) * per + blk % per) * 2 + kv;
-      const float old = low ? *sp : 0.f;
-      const int64_t stride = kv ? p.v_stride : p.k_stride;
-      const T* src = (kv ? static_cast<const T*>(p.v) : static_cast<const T*>(p.k)) +
-                     (w0 + t) * stride + (int64_t)h * kApD;
-      // V's rows are not rotated: four neighbouring dims a lane
-      const int da = kv ? 4 * lane : d.a, db = kv ? 4 * lane + 2 : d.b;
-      float x[2][8][4];
-      float amax = 0.f;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (8 * g < len) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const T* s = src + (8 * g + j < len ? 8 * g + j : 0) * stride;
-            to_vals<T>(*reinterpret_cast<const uint32_t*>(s + da),
-                       *reinterpret_cast<const uint32_t*>(s + db), x[g][j]);
-          }
-          if (!kv)
-            k_rows_f64<T>(x[g], len - 8 * g, kw, p.eps, cs64 + (t + 8 * g) * p.half, p.half, d,
-                          inter, lane);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (8 * g + j < len) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float m = fabsf(x[g][j][i]);
-                amax = fmaxf(amax, m < INFINITY ? m : 0.f);
-              }
-            }
-        }
-      }
-#pragma unroll
-      for (int m = 16; m >= 1; m >>= 1) amax = warp_max_xor(amax, m);
-      const int e_old = max(kApMinE, (int)(__float_as_uint(old) >> 23 & 0xffu) - 127);
-      int e = block_exp(amax);
-      if (low) e = max(e, e_old);
-      const float inv = pow2i(-e);
-      uint8_t* base = static_cast<uint8_t*>(kv ? p.v_cache : p.k_cache) +
-                      (blk * kApBlock * p.hkv + h) * kApD;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (8 * g + j < len) {
-            uint8_t* c = base + (slot_s[t + 1 + 8 * g + j] % kApBlock) * row;
-            const float* y = x[g][j];
-            const uint32_t w = e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-            *reinterpret_cast<uint16_t*>(c + da) = (uint16_t)w;
-            *reinterpret_cast<uint16_t*>(c + db) = (uint16_t)(w >> 16);
-          }
-        }
-      }
-      if (e > e_old && low) {  // the kept rows move to the larger scale
-        const float f = pow2i(max(e_old - e, -126));
-#pragma unroll 4
-        for (int j = 0; j < low; ++j) {
-          uint32_t* c = reinterpret_cast<uint32_t*>(base + j * row + 4 * lane);
-          float y[4];
-          e4m3x4_f32(*c, y);
-          *c = e4m3x4(y[0] * f, y[1] * f, y[2] * f, y[3] * f);
-        }
-      }
-      if (lane == 0 && (!low || e > e_old)) *sp = pow2i(e);
+    // units: (run, kv head), K then V by a pair of warps, or K and V apart by
+    // single warps
+    const int per = p.page / kApBlock, nu = nrun_s * p.hkv;
+    for (int i = kWide ? warp >> 1 : warp; i < (kWide ? nu : 2 * nu);
+         i += kWide ? kApWarps / 2 : kApWarps) {
+      const bool only_v = !kWide && i >= nu;
+      const int r = (only_v ? i - nu : i) / p.hkv, h = (only_v ? i - nu : i) % p.hkv;
+      const int t = lead_s[r];
+      Unit u;
+      u.slot = slot_s + t + 1;
+      u.len = len_s[r];
+      u.row0 = kWide ? (warp & 1) * 8 : 0;
+      const int64_t blk = u.slot[0] / kApBlock;
+      u.low = (int)(u.slot[0] % kApBlock);
+      u.row = (int64_t)p.hkv * kApD;
+      const int64_t block0 = (blk * kApBlock * p.hkv + h) * kApD;
+      float* scale = p.scale + (((blk / per) * p.hkv + h) * per + blk % per) * 2;
+      const T* ks = static_cast<const T*>(p.k) + (w0 + t) * p.k_stride + (int64_t)h * kApD;
+      const T* vs = static_cast<const T*>(p.v) + (w0 + t) * p.v_stride + (int64_t)h * kApD;
+      const double2* c64 = cs64 + t * p.half;
+      if (kWide && u.len == kApBlock)
+        unit<T, kM, kWide, true, kInter>(p, u, ks, vs, scale, block0, false, c64, d, duo_s, warp,
+                                         lane);
+      else
+        unit<T, kM, kWide, false, kInter>(p, u, ks, vs, scale, block0, only_v, c64, d, duo_s, warp,
+                                          lane);
     }
   }
 }
 
+template <typename T, bool kF8, bool kInter>
+int launch_append(const AppendParams& p, dim3 grid, size_t smem, cudaStream_t s) {
+  return launch_pdl(p.window > 1 ? rope_append_kernel<T, kF8, true, kInter>
+                                 : rope_append_kernel<T, kF8, false, kInter>,
+                    grid, dim3(kApThreads), smem, s, "rope_append launch", p);
+}
 template <typename T>
 int launch_append(const AppendParams& p, dim3 grid, size_t smem, cudaStream_t s) {
-  const bool f8 = p.scale != nullptr, wide = p.window > 1;
-  auto kern = f8 ? (wide ? rope_append_kernel<T, true, true> : rope_append_kernel<T, true, false>)
-                 : (wide ? rope_append_kernel<T, false, true> : rope_append_kernel<T, false, false>);
-  return launch_pdl(kern, grid, dim3(kApThreads), smem, s, "rope_append launch", p);
+  if (p.scale)
+    return p.inter ? launch_append<T, true, true>(p, grid, smem, s)
+                   : launch_append<T, true, false>(p, grid, smem, s);
+  return p.inter ? launch_append<T, false, true>(p, grid, smem, s)
+                 : launch_append<T, false, false>(p, grid, smem, s);
 }
 
 }  // namespace

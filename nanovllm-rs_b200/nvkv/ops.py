@@ -7,6 +7,7 @@ libnvkv.so on the current CUDA stream.  Nothing here computes on the host.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -46,14 +47,6 @@ def _row_view_ok(t: torch.Tensor) -> bool:
             return False
         exp *= t.size(d)
     return True
-
-
-def _same_device(*tensors: Optional[torch.Tensor]) -> None:
-    """Every tensor on the current cuda device, whose stream the call uses."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        _need(t is None or (t.is_cuda and t.get_device() == dev),
-              "every tensor must be on the current cuda device")
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -258,16 +251,45 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: str = "plain", factor:
     return inv_freq, a.value
 
 
-def _rope_args(positions: torch.Tensor, inv_freq: torch.Tensor, T: int) -> None:
-    _need(positions.dtype == torch.int64 and positions.is_contiguous() and
-          positions.numel() == T, "positions: contiguous int64 [T]")
-    _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
-          "inv_freq: contiguous f64 [rot_dim / 2]")
+# The calls below run per layer and step, where a decode step's kernels take a
+# few microseconds, so their checks are kept to plain attribute reads: pointers
+# go to ctypes as integers, and the raw stream is read without a Stream object.
+
+def _bad(msg: str) -> NvkvError:
+    return NvkvError(ERR_INVALID_ARG, msg)
 
 
-def _stride0(t: Optional[torch.Tensor]) -> int:
-    """Token stride in elements (a single token's is its row length)."""
-    return 0 if t is None else t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
+def _rows(t: torch.Tensor, dtype: torch.dtype) -> int:
+    """Token stride (elements) of [T, H, d] rows whose heads are dense."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or t.dtype != dtype or (st[2] != 1 and sh[2] != 1) or \
+            (st[1] != sh[2] and sh[1] != 1):
+        raise _bad("rows must be [T, H, d] of one dtype with dense heads")
+    return st[0] if sh[0] > 1 else sh[1] * sh[2]
+
+
+def _raw_stream(*tensors: Optional[torch.Tensor]) -> int:
+    """The current stream of the current device, which must hold every tensor."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            raise _bad("every tensor must be on the current cuda device")
+    if dev != torch.cuda.current_device():
+        raise _bad("every tensor must be on the current cuda device")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _rope_args(positions: torch.Tensor, inv_freq: torch.Tensor, T: int) -> int:
+    """Checks the angles' inputs; returns rot_dim."""
+    if positions.dtype != torch.int64 or positions.numel() != T or not positions.is_contiguous():
+        raise _bad("positions: contiguous int64 [T]")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise _bad("inv_freq: contiguous f64 [rot_dim / 2]")
+    return 2 * inv_freq.numel()
 
 
 def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
@@ -278,34 +300,48 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
     may be strided, k may be None): the first 2 * inv_freq.numel() dims of every
     head, half or interleaved pairs, f32 rounded once.  q_out / k_out default to
     new tensors and may be q / k (in place).  Negated positions rotate back."""
-    for t in (q, k, q_out, k_out):
-        _need(t is None or (t.dim() == 3 and _row_view_ok(t) and t.dtype == q.dtype),
-              "q / k and their outputs: [T, H, d] of one dtype, rows dense")
+    dt = q.dtype
+    qs = _rows(q, dt)
     T, hq, d = q.shape
-    _need(k is None or (k.size(0) == T and k.size(2) == d), "k must match q's tokens and head size")
-    _need(k is not None or k_out is None, "k_out without k")
-    _rope_args(positions, inv_freq, T)
+    rot = _rope_args(positions, inv_freq, T)
     if q_out is None:
-        q_out = torch.empty(T, hq, d, device=q.device, dtype=q.dtype)
-    if k is not None and k_out is None:
-        k_out = torch.empty(T, k.size(1), d, device=q.device, dtype=q.dtype)
-    _need(q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "output shape")
-    _same_device(q, k, q_out, k_out, positions, inv_freq)
-    check(lib.nvkv_rope(_ptr(q), _stride0(q), _ptr(k), _stride0(k), _ptr(q_out), _stride0(q_out),
-                        _ptr(k_out), _stride0(k_out), T, hq, 0 if k is None else k.size(1), d,
-                        _ptr(positions), _ptr(inv_freq), 2 * inv_freq.numel(), float(attn_factor),
-                        1 if interleaved else 0, _dtype(q), _stream()))
+        q_out, qos = q.new_empty(q.shape), hq * d
+    else:
+        qos = _rows(q_out, dt)
+        if q_out.shape != q.shape:
+            raise _bad("q_out must have q's shape")
+    hkv = ks = kos = 0
+    if k is not None:
+        ks, hkv = _rows(k, dt), k.size(1)
+        if k.size(0) != T or k.size(2) != d:
+            raise _bad("k must match q's tokens and head size")
+        if k_out is None:
+            k_out, kos = k.new_empty(k.shape), hkv * d
+        else:
+            kos = _rows(k_out, dt)
+            if k_out.shape != k.shape:
+                raise _bad("k_out must have k's shape")
+    elif k_out is not None:
+        raise _bad("k_out without k")
+    stream = _raw_stream(q, k, q_out, k_out, positions, inv_freq)
+    check(lib.nvkv_rope(q.data_ptr(), qs, _at(k), ks, q_out.data_ptr(), qos, _at(k_out), kos, T,
+                        hq, hkv, d, positions.data_ptr(), inv_freq.data_ptr(), rot, attn_factor,
+                        1 if interleaved else 0, _dtype(q), stream))
     return q_out, k_out
 
 
-def _fp8b_pool(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: torch.Tensor) -> None:
-    _need(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and k_cache.dim() == 4 and
-          k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.shape == k_cache.shape,
-          "fp8b caches: contiguous uint8 [Nb, P, Hkv, 128]")
-    nb, page, hkv, _ = k_cache.shape
-    _need(kv_scale.dtype == torch.float32 and kv_scale.is_contiguous() and
-          page % FP8B_BLOCK == 0 and tuple(kv_scale.shape) == (nb, hkv, page // FP8B_BLOCK, 2),
-          "kv_scale: contiguous f32 [Nb, Hkv, P / 16, 2]")
+def _fp8b_pool(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: torch.Tensor):
+    """Checks a block-scaled pool; returns its shape (Nb, P, Hkv, 128)."""
+    sh = k_cache.shape
+    if len(sh) != 4 or v_cache.shape != sh or k_cache.dtype != torch.uint8 or \
+            v_cache.dtype != torch.uint8 or not k_cache.is_contiguous() or \
+            not v_cache.is_contiguous():
+        raise _bad("fp8b caches: contiguous uint8 [Nb, P, Hkv, 128]")
+    if kv_scale.dtype != torch.float32 or sh[1] % FP8B_BLOCK or \
+            kv_scale.shape != (sh[0], sh[2], sh[1] // FP8B_BLOCK, 2) or \
+            not kv_scale.is_contiguous():
+        raise _bad("kv_scale: contiguous f32 [Nb, Hkv, P / 16, 2]")
+    return sh
 
 
 def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
@@ -321,38 +357,46 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     [Nb, P, Hkv, 128], or with kv_scale [Nb, Hkv, P / 16, 2] the block-scaled
     e4m3 pool (uint8).  Tokens of one 16-slot block must be neighbours with
     ascending slots."""
-    for t in (q, k, v, q_out):
-        _need(t is None or (t.dim() == 3 and _row_view_ok(t) and t.dtype == k.dtype),
-              "q, k, v: [T, H, 128] of one dtype, rows dense")
+    dt = k.dtype
+    ks, vs = _rows(k, dt), _rows(v, dt)
     T, hkv, d = k.shape
-    _need(v.shape == k.shape and (q is None or (q.size(0) == T and q.size(2) == d)),
-          "q, k and v must match in tokens and head size")
-    _rope_args(positions, inv_freq, T)
-    _need(slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous() and
-          slot_mapping.numel() == T, "slot_mapping: contiguous int64 [T]")
+    if v.shape != k.shape:
+        raise _bad("v must have k's shape")
+    rot = _rope_args(positions, inv_freq, T)
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T or \
+            not slot_mapping.is_contiguous():
+        raise _bad("slot_mapping: contiguous int64 [T]")
     if kv_scale is not None:
-        _fp8b_pool(k_cache, v_cache, kv_scale)
+        nb, page, ch, cd = _fp8b_pool(k_cache, v_cache, kv_scale)
     else:
-        _need(k_cache.dtype == k.dtype and v_cache.dtype == k.dtype and k_cache.dim() == 4 and
-              k_cache.is_contiguous() and v_cache.is_contiguous() and
-              v_cache.shape == k_cache.shape, "caches: contiguous [Nb, P, Hkv, 128] of k's dtype")
-    nb, page = k_cache.size(0), k_cache.size(1)
-    _need(k_cache.size(2) == hkv and k_cache.size(3) == d, "cache rows must match k")
+        if k_cache.dtype != dt or v_cache.dtype != dt or k_cache.dim() != 4 or \
+                v_cache.shape != k_cache.shape or not k_cache.is_contiguous() or \
+                not v_cache.is_contiguous():
+            raise _bad("caches: contiguous [Nb, P, Hkv, 128] of k's dtype")
+        nb, page, ch, cd = k_cache.shape
+    if ch != hkv or cd != d:
+        raise _bad("cache rows must match k")
     for w in (q_norm_w, k_norm_w):
-        _need(w is None or (w.dtype == k.dtype and w.is_contiguous() and w.numel() == d),
-              "norm weights: [128] of k's dtype")
-    _need(q is not None or q_out is None, "q_out without q")
-    if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    _need(q is None or (q_out.shape == q.shape and q_out.is_contiguous()), "q_out: contiguous")
-    _same_device(q, k, v, q_out, positions, inv_freq, k_cache, v_cache, kv_scale, slot_mapping,
-                 q_norm_w, k_norm_w)
+        if w is not None and (w.dtype != dt or w.numel() != d or not w.is_contiguous()):
+            raise _bad("norm weights: [128] of k's dtype")
+    hq = qs = 0
+    if q is not None:
+        qs, hq = _rows(q, dt), q.size(1)
+        if q.size(0) != T or q.size(2) != d:
+            raise _bad("q must match k's tokens and head size")
+        if q_out is None:
+            q_out = q.new_empty(q.shape)
+        elif q_out.shape != q.shape or q_out.dtype != dt or not q_out.is_contiguous():
+            raise _bad("q_out: contiguous, like q")
+    elif q_out is not None:
+        raise _bad("q_out without q")
+    stream = _raw_stream(k, v, q, q_out, positions, inv_freq, k_cache, v_cache, kv_scale,
+                         slot_mapping, q_norm_w, k_norm_w)
     check(lib.nvkv_rope_append(
-        _ptr(q), _stride0(q), _ptr(k), _stride0(k), _ptr(v), _stride0(v), T,
-        0 if q is None else q.size(1), hkv, d, _ptr(positions), _ptr(inv_freq),
-        2 * inv_freq.numel(), float(attn_factor), 1 if interleaved else 0, _ptr(q_norm_w),
-        _ptr(k_norm_w), float(eps), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(kv_scale),
-        _ptr(slot_mapping), nb, page, _dtype(k), _stream()))
+        _at(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, hq, hkv, d, positions.data_ptr(),
+        inv_freq.data_ptr(), rot, attn_factor, 1 if interleaved else 0, _at(q_norm_w),
+        _at(k_norm_w), eps, _at(q_out), k_cache.data_ptr(), v_cache.data_ptr(), _at(kv_scale),
+        slot_mapping.data_ptr(), nb, page, _dtype(k), stream))
     return q_out
 
 
@@ -363,25 +407,25 @@ def load_kvcache_fp8b(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: to
     """Rows `slots` [n] int64 of the block-scaled e4m3 pool as (k, v)
     [n, Hkv, 128] bf16 / f16 (nvkv_load_kvcache_fp8b); negative slots give
     zeros."""
-    _fp8b_pool(k_cache, v_cache, kv_scale)
-    nb, page, hkv, d = k_cache.shape
-    _need(slots.dtype == torch.int64 and slots.dim() == 1 and slots.is_contiguous(),
-          "slots: contiguous int64 [n]")
+    nb, page, hkv, d = _fp8b_pool(k_cache, v_cache, kv_scale)
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise _bad("slots: contiguous int64 [n]")
     n = slots.numel()
     if k_out is None:
-        k_out = torch.empty(n, hkv, d, device=k_cache.device, dtype=dtype)
+        k_out = k_cache.new_empty((n, hkv, d), dtype=dtype)
     if v_out is None:
-        v_out = torch.empty(n, hkv, d, device=k_cache.device, dtype=dtype)
+        v_out = k_out.new_empty((n, hkv, d))
     for t in (k_out, v_out):
-        _need(tuple(t.shape) == (n, hkv, d) and t.is_contiguous() and t.dtype == k_out.dtype,
-              "outputs: contiguous [n, Hkv, 128] of one dtype")
-    _same_device(k_cache, v_cache, kv_scale, slots, k_out, v_out)
-    check(lib.nvkv_load_kvcache_fp8b(_ptr(k_cache), _ptr(v_cache), _ptr(kv_scale), _ptr(slots), n,
-                                     hkv, d, nb, page, _ptr(k_out), _ptr(v_out), _dtype(k_out),
-                                     _stream()))
+        if t.shape != (n, hkv, d) or t.dtype != k_out.dtype or not t.is_contiguous():
+            raise _bad("outputs: contiguous [n, Hkv, 128] of one dtype")
+    stream = _raw_stream(k_cache, v_cache, kv_scale, slots, k_out, v_out)
+    check(lib.nvkv_load_kvcache_fp8b(k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(),
+                                     slots.data_ptr(), n, hkv, d, nb, page, k_out.data_ptr(),
+                                     v_out.data_ptr(), _dtype(k_out), stream))
     return k_out, v_out
 
 
+@functools.lru_cache(maxsize=256)
 def workspace_size_fp8b(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_seqlen_q: int,
                         max_seqlen_k: int, prompt_kv_tokens: int = 0, head_dim: int = 128) -> int:
     n = ctypes.c_size_t(0)
@@ -389,6 +433,9 @@ def workspace_size_fp8b(num_seqs: int, num_q_heads: int, num_kv_heads: int, max_
                                                        head_dim, max_seqlen_q, max_seqlen_k,
                                                        int(prompt_kv_tokens), ctypes.byref(n)))
     return n.value
+
+
+_INT32 = (torch.int32, torch.uint32)
 
 
 def paged_attention_fp8b(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -401,33 +448,35 @@ def paged_attention_fp8b(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """paged_attention over the block-scaled e4m3 pool (nvkv_paged_attention_fp8b).
     prompt_kv_tokens: at least the sum of k_len over the q_len > 1 sequences,
     needed when max_seqlen_q * Hq / Hkv > 32."""
-    _need(q.dim() == 3 and _row_view_ok(q), "q must be [T, Hq, D], rows dense")
-    _fp8b_pool(k_cache, v_cache, kv_scale)
-    _need(block_tables.dim() == 2 and block_tables.is_contiguous() and
-          block_tables.dtype in (torch.int32, torch.uint32), "block_tables: contiguous 32-bit [B, W]")
-    for t in (cu_seqlens_q, cu_seqlens_k):
-        _need(t.dtype in (torch.int32, torch.uint32) and t.is_contiguous() and t.numel() >= 1 and
-              t.numel() == cu_seqlens_q.numel(), "cu_seqlens: contiguous 32-bit [B + 1]")
+    dt = q.dtype
+    qs = _rows(q, dt)
     T, hq, d = q.shape
-    nb, page, hkv = k_cache.size(0), k_cache.size(1), k_cache.size(2)
+    nb, page, hkv, cd = _fp8b_pool(k_cache, v_cache, kv_scale)
     B = cu_seqlens_q.numel() - 1
-    _need(block_tables.size(0) >= B and k_cache.size(3) == d, "one block_tables row a sequence")
+    if block_tables.dtype not in _INT32 or block_tables.dim() != 2 or \
+            block_tables.size(0) < B or not block_tables.is_contiguous():
+        raise _bad("block_tables: contiguous 32-bit, one row a sequence")
+    if cu_seqlens_q.dtype not in _INT32 or cu_seqlens_k.dtype not in _INT32 or B < 0 or \
+            cu_seqlens_k.numel() != B + 1 or not cu_seqlens_q.is_contiguous() or \
+            not cu_seqlens_k.is_contiguous():
+        raise _bad("cu_seqlens: contiguous 32-bit [B + 1]")
+    if cd != d:
+        raise _bad("cache rows must match q")
     if out is None:
-        out = torch.empty(T, hq, d, device=q.device, dtype=q.dtype)
-    _need(out.shape == q.shape and out.is_contiguous() and out.dtype == q.dtype,
-          "out: contiguous, like q")
+        out = q.new_empty(q.shape)
+    elif out.shape != q.shape or out.dtype != dt or not out.is_contiguous():
+        raise _bad("out: contiguous, like q")
     need = workspace_size_fp8b(B, hq, hkv, max_seqlen_q, max_seqlen_k, prompt_kv_tokens, d)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _same_device(q, k_cache, v_cache, kv_scale, cu_seqlens_q, cu_seqlens_k, block_tables, out,
-                 workspace)
+    if ws_bytes < need:
+        workspace, ws_bytes = k_cache.new_empty(need), need
+    stream = _raw_stream(q, k_cache, v_cache, kv_scale, cu_seqlens_q, cu_seqlens_k, block_tables,
+                         out, workspace)
     check(lib.nvkv_paged_attention_fp8b(
-        _ptr(q), _stride0(q), T, _ptr(k_cache), _ptr(v_cache), _ptr(kv_scale), nb, _ptr(out),
-        _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), _ptr(block_tables), block_tables.size(1), B,
-        int(max_seqlen_q), int(max_seqlen_k), hq, hkv, d, page, float(softmax_scale),
-        1 if causal else 0, int(prompt_kv_tokens), _ptr(workspace), ws_bytes, _dtype(q),
-        _stream()))
+        q.data_ptr(), qs, T, k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(), nb,
+        out.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
+        block_tables.size(1), B, max_seqlen_q, max_seqlen_k, hq, hkv, d, page, softmax_scale,
+        1 if causal else 0, prompt_kv_tokens, _at(workspace), ws_bytes, _dtype(q), stream))
     return out
 
 
