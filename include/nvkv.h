@@ -329,7 +329,8 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * does not fit is skipped and recorded as NVKV_DEVERR_SEQLEN).  Malformed
  * sequences are skipped and recorded as in nvkv_paged_attention.  Products
  * are exact in the codes: queries enter as three e4m3 pieces (12 significant
- * bits), the softmax weights as three (2^-12 of a weight), sums in f32.  Calls
+ * bits), the softmax weights as four (2^-12 of a weight down to 2^-17 of the
+ * row's largest), sums in f32.  Calls
  * that may overlap on the GPU need a workspace each.
  * ---------------------------------------------------------------------- */
 #define NVKV_FP8B_BLOCK 16 /* slots that share a scale */

@@ -124,7 +124,7 @@ int launch_prompt_rows(const uint32_t* cu_q, const uint32_t* cu_k, int num_seqs,
 // `all` says that every sequence should be such a one.
 constexpr int kFp8bMaxRows = 32;
 int launch_decode_fp8b(const AttnArgs& a, int q_cap, bool all);
-size_t decode_fp8b_bytes(int num_seqs, int hq, int hkv, int max_k, int q_cap);
+size_t decode_fp8b_bytes(int hq, int hkv, int q_cap);
 // Bytes of the prefill work plan (0 when max_seqlen_q <= 1); it sits in the
 // attention workspace after the decode scratch, at attention_plan_offset().
 size_t prefill_plan_bytes(int num_seqs, int max_seqlen_q);

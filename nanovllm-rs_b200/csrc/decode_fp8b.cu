@@ -1,26 +1,23 @@
 // Decode attention over the block-scaled e4m3 pool, on tcgen05 (sequences of a
 // few query tokens: rows = q_len x (Hq / Hkv) <= 32).
 //
-// Work item = (split, kv head, sequence): a CTA streams one chunk of one
-// sequence's keys for one kv head, 128 keys a tile, and serves all its rows, so
-// every code leaves HBM once.  Both products run on the tensor cores with the
+// A CTA streams a sequence's keys for one kv head, 128 keys a tile, and serves all
+// its rows, so every code leaves HBM once.  Both products run on the tensor cores with the
 // codes exactly as TMA put them into shared memory -- nothing is converted:
 //   S^T [128 keys x rows] = K codes (A, K-major) . Q^T (B)
 //   O^T [128 dims x rows] += V codes^T (A, MN-major) . P^T (B)
-// Q and the weights P enter as THREE e4m3 pieces each, x = c0 + 2^-5 c1 +
-// 2^-10 c2, every piece the e4m3 rounding of what the ones before left over
-// (c0's error is at most 8 of a value below 256, so 32 times it fits again);
-// together they hold 12 significant bits.  The pieces are extra columns of B
-// (the tensor core's N has room: 3 x rows), and are joined in f32 with their
-// weights where the columns are read.
+// Q enters as three e4m3 pieces, the weights P as four, every piece the e4m3
+// rounding of what the ones before left over.  The pieces are extra columns of B
+// (the tensor core's N has room), and are joined in f32 with their weights where
+// the columns are read.
 //
 // A compute thread owns one key of the tile (one TMEM lane): it joins its
 // scores, multiplies by the key block's K scale, and forms z = S + log2(V
 // scale), so a weight 2^(z - M) already carries the value's scale and O needs
-// none; the row sum takes the scale back out (an exact power of two).  M is the
-// running maximum of z per row over the CTA's keys: warp maxima by redux.sync,
-// joined over the four warps through shared memory with one named barrier a
-// tile.  When M grows the threads rescale O in TMEM.  Weights leave as one or
+// none; the row sum takes the scale back out (an exact power of two).  M is a
+// row's maximum of z over the CTA's keys, to within a headroom: warp maxima by
+// redux.sync, joined over the four warps through shared memory with one named
+// barrier a tile; when M moves the threads rescale O in TMEM.  Weights leave as one or
 // more 16-byte stores a thread (N-major B operand).
 //
 //   warps 0-3  compute (TMEM lanes 32 w .. 32 w + 31)
@@ -29,6 +26,16 @@
 //   warp 5     TMEM allocation and every tcgen05.mma, one thread, in the order
 //              S(0), S(1), O(0), S(2), O(1), ...: a tile's scores are computed
 //              while the tile before it is in the softmax
+//   warps 6-7  the next sequence's Q pieces
+//
+// Work.  One wave of persistent CTAs, a group of Hkv neighbours (one per kv head)
+// for each share of the batch: the sequences' tiles, one after the other, are cut
+// into equal shares wherever the cuts fall, so every SM has the same number of
+// tiles whatever the lengths, and ring, tensor memory and barriers are set up
+// once.  (A CTA per (split, head, sequence) lost ~6 us of its 14 to its start and
+// end.)  A share's whole sequences are written out; of a sequence that a cut goes
+// through, each CTA leaves f32 partials and a base-2 log-sum-exp in the workspace
+// (at most two per CTA), and combine_fp8b_kernel joins them.
 //
 // Bound by HBM: 2 x 128 bytes of codes + 0.5 of scales a key and kv head; per
 // tile the compute warps issue ~700 instructions for 32 KB.
@@ -45,27 +52,42 @@ constexpr int kBTile = 128;                   // keys a tile
 constexpr int kBCode = kBTile * kBD;          // 16 KB of codes
 constexpr int kBStage = 2 * kBCode;           // K, V
 constexpr int kBScale = kBTile / NVKV_FP8B_BLOCK * 2;  // floats of a tile's scales
-constexpr int kBThreads = 192;
+constexpr int kBThreads = 256;
 constexpr float kLog2e_ = 1.4426950408889634f;
-constexpr float kPiece1 = 1.f / 32.f, kPiece2 = 1.f / 1024.f;  // weights of pieces 1 and 2
+// Q and the weights P as sums of e4m3 pieces, x = c0 + 2^-5 c1 + 2^-10 c2 + ...,
+// every piece the e4m3 rounding of what the ones before left over (at most 8 of a
+// value below 256, so 32 times it fits again): 4 more bits each.
+constexpr int kQPieces = 3, kPPieces = 4;
+constexpr float kPiece1 = 1.f / 32.f, kPiece2 = 1.f / 1024.f, kPiece3 = 1.f / 32768.f;
+// M is kept until a row's maximum passes it by this much (weights then reach 2^3):
+// rescaling O waits for the product before it, and with M exact more than half of
+// the first ten tiles of random scores did so.  Weights enter the pieces times
+// 2^(8 - 3), so that the largest is 256; a weight down to 2^-17 of the largest
+// keeps 12 bits.  (Three pieces, which the same number of columns would do for 4
+// and 8 rows, keep 9 bits at 2^-15: too few where one key takes nearly all of the
+// weight and the answer lies in the others.)
+constexpr float kHeadroom = 3.f;
+constexpr float kWeight = 32.f;
 
 // Rows a CTA serves, padded: 4, 8, 16 or 32; its resources by that.
 template <int HP>
 struct Cfg {
-  static constexpr int kCols = (3 * HP + 15) / 16 * 16;       // pieces as B columns
+  static constexpr int kCols = (kQPieces * HP + 15) / 16 * 16;  // pieces as B columns
+  static constexpr int kPCols = kPPieces * HP;
   static constexpr int kCtasPerSm = HP <= 8 ? 2 : 1;
   static constexpr int kStages = HP <= 8 ? 3 : HP == 16 ? 6 : 5;
+  static constexpr int kQBufs = HP == 8 ? 1 : 2;
   static constexpr int kQBytes = kCols * 128;
-  static constexpr int kPBytes = kCols * 128;                 // one of two buffers
-  static constexpr int kTmem = 3 * kCols <= 64 ? 64 : 3 * kCols <= 128 ? 128
-                               : 3 * kCols <= 256 ? 256 : 512;
+  static constexpr int kPBytes = kPCols * 128;  // one of two buffers
+  static constexpr int kUsed = 2 * kCols + kPCols;  // tensor-memory columns: two S, one O
+  static constexpr int kTmem = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static constexpr int kOffQ = kStages * kBStage;
-  static constexpr int kOffP = kOffQ + kQBytes;
+  static constexpr int kOffP = kOffQ + kQBufs * kQBytes;
   static constexpr int kOffScale = kOffP + 2 * kPBytes;
   static constexpr int kOffRed = kOffScale + kStages * kBScale * 4;  // [2][4][HP] maxima
-  static constexpr int kOffRow = kOffRed + 2 * 4 * HP * 4;           // [HP] factor, [HP] limit
-  static constexpr int kOffBar = kOffRow + 2 * HP * 4;
-  static constexpr int kBars = 2 * kStages + 8;
+  static constexpr int kOffRow = kOffRed + 2 * 4 * HP * 4;           // [2][HP] factors, [HP] limits
+  static constexpr int kOffBar = kOffRow + 3 * HP * 4;
+  static constexpr int kBars = 2 * kStages + 11;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
   static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "decode fp8b: CTAs per SM");
   static_assert(kCtasPerSm * kTmem <= 512, "decode fp8b: tensor memory per SM");
@@ -78,10 +100,79 @@ struct Params {
   const uint32_t *cu_q, *cu_k, *block_tables;
   int64_t bt_stride, num_blocks, num_q_rows;
   const float* scale;
-  int hq, hkv, group, page, chunk, max_k, max_splits, q_cap, all, causal;
+  int num_seqs, hq, hkv, group, groups, page, max_k, q_cap, all, causal;
   float scale_log2;
-  float *ws_o, *ws_lse;  // [B][splits][hkv][q_cap * group] (x 128)
+  // partials: slot 2 cta (a sequence that began in an earlier share) and 2 cta + 1
+  // (one that goes on in a later share)
+  int2* ws_desc;         // [2 ctas] {sequence or -1, 1: the sequence's last part}
+  float *ws_lse, *ws_o;  // [2 ctas][q_cap * group] (x 128)
   int* err;
+};
+
+// A sequence as the kernel sees it.
+struct Seq {
+  uint32_t q0;
+  int q_len, k_len, tiles;
+};
+// tiles = 0: nothing to do (another kernel's, or malformed: *err then gets a code
+// if it is not null).  zero: rows without keys, whose output is 0.
+__device__ __forceinline__ Seq read_seq(const Params& p, int b, int* err, bool* zero) {
+  Seq s;
+  s.q0 = p.cu_q[b];
+  s.q_len = (int)(p.cu_q[b + 1] - s.q0);
+  s.k_len = (int)(p.cu_k[b + 1] - p.cu_k[b]);
+  s.tiles = 0;
+  const bool other = s.q_len < 0 || s.q_len > p.q_cap;
+  if (s.q_len == 0 || (other && !p.all)) return s;
+  if (other || s.k_len > p.max_k || (int64_t)s.q0 + s.q_len > p.num_q_rows ||
+      (s.q_len > 1 && s.k_len < s.q_len)) {
+    if (err) record_error(err, NVKV_DEVERR_SEQLEN);
+    return s;
+  }
+  if (s.k_len <= 0) {
+    if (err) record_error(err, NVKV_DEVERR_SEQLEN);
+    if (zero) *zero = true;
+    return s;
+  }
+  s.tiles = (s.k_len + kBTile - 1) / kBTile;
+  return s;
+}
+
+// A warp's walk over the share's sequences: lane i holds sequence base + i.
+struct Cursor {
+  Seq mine;
+  int base, b, t, left;  // sequence, its first tile here, tiles left of the share
+  __device__ __forceinline__ void fill(const Params& p, int lane) {
+    base = b;
+    mine.tiles = 0;
+    if (b + lane < p.num_seqs) mine = read_seq(p, b + lane, nullptr, nullptr);
+  }
+  __device__ __forceinline__ void start(const Params& p, int b0, int t0, int n, int lane) {
+    b = b0;
+    t = t0;
+    left = n;
+    fill(p, lane);
+  }
+  // the next part: false when the share is done
+  __device__ __forceinline__ bool next(const Params& p, Seq& s, int& n, int lane) {
+    if (left <= 0) return false;
+    for (;;) {
+      if (b - base >= 32) fill(p, lane);
+      s.tiles = __shfl_sync(0xffffffffu, mine.tiles, b - base);
+      if (s.tiles > 0 || b >= p.num_seqs) break;
+      ++b;
+    }
+    s.q0 = __shfl_sync(0xffffffffu, mine.q0, b - base);
+    s.q_len = __shfl_sync(0xffffffffu, mine.q_len, b - base);
+    s.k_len = __shfl_sync(0xffffffffu, mine.k_len, b - base);
+    n = min(s.tiles - t, left);
+    left -= n;
+    return n > 0;
+  }
+  __device__ __forceinline__ void advance() {
+    ++b;
+    t = 0;
+  }
 };
 
 __device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -148,13 +239,14 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
       : "r"(w));
   return DT<__half>::to_f2(h);
 }
-// Four values (0 <= |x| <= 256) as three pieces: w[p] = the codes of piece p.
-__device__ __forceinline__ void pieces4(float a, float b, float c, float d, uint32_t (&w)[3]) {
+// Four values (0 <= |x| <= 256) as N pieces: w[p] = the codes of piece p.
+template <int N>
+__device__ __forceinline__ void pieces4(float a, float b, float c, float d, uint32_t (&w)[N]) {
 #pragma unroll
-  for (int p = 0; p < 3; ++p) {
+  for (int p = 0; p < N; ++p) {
     const uint32_t lo = e4m3x2(a, b), hi = e4m3x2(c, d);
     w[p] = lo | (hi << 16);
-    if (p < 2) {
+    if (p < N - 1) {
       const float2 x = e4m3x2_f32(lo), y = e4m3x2_f32(hi);
       a = (a - x.x) * 32.f;
       b = (b - x.y) * 32.f;
@@ -167,24 +259,20 @@ __device__ __forceinline__ void pieces4(float a, float b, float c, float d, uint
 // The rows' queries as B of the first product: row p HP + r of Q (128 bytes,
 // SWIZZLE_128B) holds piece p of q row r times a power of two that puts the
 // row's largest |q| into [128, 256); rowf[r] undoes it (times the softmax
-// scale).  Missing rows are zero.
+// scale).  Rows past `rows` are zero.  Two warps (w = 0, 1).
 template <typename T, int HP>
 __device__ __forceinline__ void load_q(const Params& p, uint32_t q0, int kvh, int rows,
-                                       uint8_t* sq, float* rowf, int warp, int lane) {
-  constexpr int kCols = Cfg<HP>::kCols;
-  for (int i = threadIdx.x; i < kCols * 8; i += 128)
-    *reinterpret_cast<uint4*>(sq + i * 16) = make_uint4(0, 0, 0, 0);
-  bar_compute();
-  for (int r = warp; r < HP; r += 4) {
-    if (r >= rows) {
-      if (lane == 0) rowf[r] = 0.f;
-      continue;
+                                       uint8_t* sq, float* rowf, int w, int lane) {
+#pragma unroll 4
+  for (int r = w; r < HP; r += 2) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < rows) {
+      const T* src = static_cast<const T*>(p.q) + (int64_t)(q0 + r / p.group) * p.q_stride +
+                     (int64_t)(kvh * p.group + r % p.group) * kBD + 4 * lane;
+      const uint2 raw = *reinterpret_cast<const uint2*>(src);
+      const float2 u = DT<T>::to_f2(raw.x), v = DT<T>::to_f2(raw.y);
+      x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
     }
-    const T* src = static_cast<const T*>(p.q) + (int64_t)(q0 + r / p.group) * p.q_stride +
-                   (int64_t)(kvh * p.group + r % p.group) * kBD + 4 * lane;
-    const uint2 raw = *reinterpret_cast<const uint2*>(src);
-    const float2 u = DT<T>::to_f2(raw.x), v = DT<T>::to_f2(raw.y);
-    float x[4] = {u.x, u.y, v.x, v.y};
     float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
     m = redux_max(m);
     const int e = (int)(__float_as_uint(m) >> 23);
@@ -193,13 +281,13 @@ __device__ __forceinline__ void load_q(const Params& p, uint32_t q0, int kvh, in
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // an infinite query gives NaN, as its scores would
       x[i] = fabsf(x[i]) < INFINITY ? x[i] * up : __int_as_float(0x7fffffff);
-    uint32_t w[3];
-    pieces4(x[0], x[1], x[2], x[3], w);
+    uint32_t c[kQPieces];
+    pieces4(x[0], x[1], x[2], x[3], c);
 #pragma unroll
-    for (int pc = 0; pc < 3; ++pc) {
+    for (int pc = 0; pc < kQPieces; ++pc) {
       const int n = pc * HP + r;
       *reinterpret_cast<uint32_t*>(sq + n * 128 + (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4) =
-          w[pc];
+          c[pc];
     }
     if (lane == 0) rowf[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * p.scale_log2;
   }
@@ -219,17 +307,20 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
   float* ssc = reinterpret_cast<float*>(smem + C::kOffScale);
   float* red = reinterpret_cast<float*>(smem + C::kOffRed);
   float* rowf = reinterpret_cast<float*>(smem + C::kOffRow);
-  int* rowlim = reinterpret_cast<int*>(rowf + HP);
+  int* rowlim = reinterpret_cast<int*>(rowf + 2 * HP);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* empty = full + kStages;
   uint64_t* s_full = empty + kStages;  // [2] scores of a tile are in TMEM
   uint64_t* p_full = s_full + 2;       // [2] scores read, weights in shared memory, O rescaled
   uint64_t* o_done = p_full + 2;       // [2] the tile's O product has finished
-  uint64_t* q_full = o_done + 2;
-  uint64_t* drain = q_full + 1;
+  uint64_t* q_full = o_done + 2;       // [2] a sequence's Q pieces and row factors
+  uint64_t* q_empty = q_full + 2;      // [2] its last scores are done, its factors read
+  uint64_t* drain = q_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  __shared__ int64_t sums[9];
+  __shared__ int start_b, start_t;
 
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int cta = blockIdx.x, share = cta / p.hkv, kvh = cta % p.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 128) {
     tma_prefetch_desc(&tmap_k);
@@ -246,146 +337,216 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[x], 128);
       mbar_init(&o_done[x], 1);
+      mbar_init(&q_full[x], 64);
+      mbar_init(&q_empty[x], 129);
     }
-    mbar_init(q_full, 128);
     mbar_init(drain, 1);
     fence_mbar_init();
   }
+  for (int i = threadIdx.x; i < C::kQBufs * C::kQBytes / 16; i += kBThreads)  // the unused columns
+    *reinterpret_cast<uint4*>(sq + i * 16) = make_uint4(0, 0, 0, 0);
   pdl_wait();  // inputs may come from the kernel before this one
 
-  // the chunk's first 32 block-table entries, beside the lengths (in the row:
-  // split * chunk < the plan's bound <= page * bt_stride)
-  const int pg_first = (int)((int64_t)split * p.chunk / p.page);
-  uint32_t ent = 0;
-  if (warp == 4 && pg_first + lane < p.bt_stride)
-    ent = __ldg(p.block_tables + (int64_t)b * p.bt_stride + pg_first + lane);
-  const uint32_t q0 = p.cu_q[b];
-  const int q_len = (int)(p.cu_q[b + 1] - q0);
-  const int k_len = (int)(p.cu_k[b + 1] - p.cu_k[b]);
-  if (q_len == 0) return;
-  const bool other = q_len < 0 || q_len > p.q_cap;
-  if (other && !p.all) return;  // the prefill kernel's
-  const int nsplit = k_len > 0 ? (k_len + p.chunk - 1) / p.chunk : 1;
-  if (other || k_len > p.max_k || (int64_t)q0 + q_len > p.num_q_rows ||
-      (q_len > 1 && k_len < q_len)) {
-    if (threadIdx.x == 0) record_error(p.err, NVKV_DEVERR_SEQLEN);
-    return;
+  // ---- this CTA's share of the tiles: [lo, hi) of their total ----
+  const int each = (p.num_seqs + kBThreads - 1) / kBThreads;  // sequences a thread
+  const int b_lo = threadIdx.x * each, b_hi = min(b_lo + each, p.num_seqs);
+  int64_t mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    bool zero = false;
+    const Seq s = read_seq(p, b, cta == 0 ? p.err : nullptr, &zero);
+    mine += s.tiles;
+    if (zero && share == 0)
+      for (int r = 0; r < s.q_len * p.group; ++r) {
+        uint4* o = reinterpret_cast<uint4*>(
+            static_cast<T*>(p.out) +
+            ((int64_t)(s.q0 + r / p.group) * p.hq + kvh * p.group + r % p.group) * kBD);
+        for (int i = 0; i < kBD / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
+      }
   }
-  if (split >= nsplit) return;
-  if (k_len <= 0 && threadIdx.x == 0) record_error(p.err, NVKV_DEVERR_SEQLEN);
-  const int tok0 = split * p.chunk;
-  const int tok1 = min(k_len, tok0 + p.chunk);
-  const int ntiles = tok1 > tok0 ? (tok1 - tok0 + kBTile - 1) / kBTile : 0;
-  const int rows = q_len * p.group;
+  int64_t upto = mine;  // inclusive prefix sum over the threads
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kBThreads / 32; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+  }
+  const int64_t used = min((int64_t)p.groups, total);  // shares of at least a tile
+  if (threadIdx.x < 2) p.ws_desc[2 * cta + threadIdx.x] = make_int2(-1, 0);
+  if (share >= used) return;
+  const int64_t lo = total * share / used, hi = total * (share + 1) / used;
+  if (upto - mine <= lo && lo < upto) {  // the thread whose sequences hold the first tile
+    int64_t at = upto - mine;
+    for (int b = b_lo;; ++b) {
+      const int n = read_seq(p, b, nullptr, nullptr).tiles;
+      if (lo < at + n) {
+        start_b = b;
+        start_t = (int)(lo - at);
+        break;
+      }
+      at += n;
+    }
+  }
   if (warp == 5) {
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
+  fence_async_smem();  // Q's zeros
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // only now, with this CTA's tensor memory in hand, may the next grid start
   pdl_launch_dependents();
+  Cursor cur;
+  cur.start(p, start_b, start_t, (int)(hi - lo), lane);
+  Seq sq_info;
+  int n_tiles;
 
   if (warp == 4) {
     // ------------------------------ TMA producer ------------------------------
-    int base = 0;  // chunk page of lane 0's entry
     int it = 0, go = 1;
-    for (; it < ntiles; ++it) {
-      const int s = it % kStages;
-      const int j0 = tok0 + it * kBTile;
-      const int pi = j0 / p.page - pg_first;
-      if (pi >= base + 32) {  // warp-uniform: the next 32 entries
-        base += 32;
-        const int pg = pg_first + base + lane;
-        ent = pg < p.bt_stride ? __ldg(p.block_tables + (int64_t)b * p.bt_stride + pg) : 0u;
-      }
-      uint32_t page = __shfl_sync(0xffffffffu, ent, pi - base);
-      if ((int64_t)page >= p.num_blocks) {  // recorded; read as page 0 so that the rest finishes
-        if (lane == 0) record_error(p.err, NVKV_DEVERR_BLOCK_RANGE);
-        page = 0;
-      }
-      if (lane == 0) {
-        go = it < kStages || mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, p.err);
-        if (go) {
-          const int off = j0 % p.page;
-          const int row = (int)((int64_t)page * p.page + off);
-          uint8_t* st = smem + s * kBStage;
-          mbar_arrive_expect_tx(&full[s], kBStage + kBScale * 4);
-          tma_load_3d(st, &tmap_k, &full[s], 0, kvh, row);
-          tma_load_3d(st + kBCode, &tmap_v, &full[s], 0, kvh, row);
-          bulk_load(ssc + s * kBScale,
-                    p.scale + (((int64_t)page * p.hkv + kvh) * (p.page / NVKV_FP8B_BLOCK) +
-                               off / NVKV_FP8B_BLOCK) * 2,
-                    kBScale * 4, &full[s]);
+    while (go && cur.next(p, sq_info, n_tiles, lane)) {
+      const uint32_t* row_bt = p.block_tables + (int64_t)cur.b * p.bt_stride;
+      int base = cur.t * kBTile / p.page;  // page of lane 0's entry
+      uint32_t ent = base + lane < p.bt_stride ? __ldg(row_bt + base + lane) : 0u;
+      for (int i = 0; i < n_tiles; ++i, ++it) {
+        const int s = it % kStages;
+        const int j0 = (cur.t + i) * kBTile;
+        const int pg = j0 / p.page;
+        if (pg >= base + 32) {  // warp-uniform: the next 32 entries
+          base = pg;
+          ent = base + lane < p.bt_stride ? __ldg(row_bt + base + lane) : 0u;
         }
+        uint32_t page = __shfl_sync(0xffffffffu, ent, pg - base);
+        if ((int64_t)page >= p.num_blocks) {  // recorded; read as page 0 so that the rest finishes
+          if (lane == 0) record_error(p.err, NVKV_DEVERR_BLOCK_RANGE);
+          page = 0;
+        }
+        if (lane == 0) {
+          go = it < kStages || mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, p.err);
+          if (go) {
+            const int off = j0 - pg * p.page;
+            const int row = (int)((int64_t)page * p.page + off);
+            uint8_t* st = smem + s * kBStage;
+            mbar_arrive_expect_tx(&full[s], kBStage + kBScale * 4);
+            tma_load_3d(st, &tmap_k, &full[s], 0, kvh, row);
+            tma_load_3d(st + kBCode, &tmap_v, &full[s], 0, kvh, row);
+            bulk_load(ssc + s * kBScale,
+                      p.scale + (((int64_t)page * p.hkv + kvh) * (p.page / NVKV_FP8B_BLOCK) +
+                                 off / NVKV_FP8B_BLOCK) * 2,
+                      kBScale * 4, &full[s]);
+          }
+        }
+        go = __shfl_sync(0xffffffffu, go, 0);
+        if (!go) break;
       }
-      go = __shfl_sync(0xffffffffu, go, 0);
-      if (!go) break;
+      cur.advance();
     }
     if (!go && lane == 0)  // given up: wait for the copies in flight
       for (int i = max(0, it - kStages); i < it; ++i)
         mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err);
   } else if (warp == 5) {
     // ------------------------------- MMA issuer -------------------------------
-    if (lane == 0 && ntiles > 0) {
-      constexpr uint32_t id_s = idesc_f8(kCols, 0, 0), id_o = idesc_f8(kCols, 1, 1);
-      const uint32_t tiles = smem_u32(smem), aq = smem_u32(sq), ap = smem_u32(sp);
-      bool ok = mbar_wait(q_full, 0, p.err);
-      int it = 0;
-      for (; ok && it <= ntiles; ++it) {
-        if (it < ntiles) {  // S(it): K-major codes, 32 dims a step
-          ok = mbar_wait(&full[it % kStages], (it / kStages) & 1, p.err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ak = tiles + (it % kStages) * kBStage;
+    constexpr uint32_t id_s = idesc_f8(kCols, 0, 0), id_o = idesc_f8(C::kPCols, 1, 1);
+    const uint32_t tiles = smem_u32(smem), aq = smem_u32(sq), ap = smem_u32(sp);
+    int it = 0, part = 0;
+    bool ok = true, fresh = false;  // fresh: tile it - 1 was its part's first
+    // O += V^T . P of tile o: 32 keys a step
+    auto issue_o = [&](int o, bool first) {
+      ok = ok && mbar_wait(&p_full[o & 1], (o >> 1) & 1, p.err);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t av = tiles + (o % kStages) * kBStage + kBCode;
+      const uint32_t pb = ap + (o & 1) * C::kPBytes;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8(tmem + (it & 1) * kCols, sdesc(ak + kk * 32, 16, 1024),
-                   sdesc(aq + kk * 32, 16, 1024), id_s, kk > 0);
-          tc_commit(&s_full[it & 1]);
-        }
-        if (it > 0) {  // O += V^T . P of the tile before: 32 keys a step
-          const int o = it - 1;
-          ok = mbar_wait(&p_full[o & 1], (o >> 1) & 1, p.err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t av = tiles + (o % kStages) * kBStage + kBCode;
-          const uint32_t pb = ap + (o & 1) * C::kPBytes;
+      for (int kk = 0; kk < 4; ++kk)
+        mma_f8(tmem + 2 * kCols, sdesc(av + kk * 32 * 128, 16, 1024),
+               sdesc_plain(pb + kk * 512, 128, 2048), id_o, !first || kk > 0);
+      tc_commit(&o_done[o & 1]);
+      tc_commit(&empty[o % kStages]);
+    };
+    while (cur.next(p, sq_info, n_tiles, lane)) {
+      if (lane == 0) {
+        const int qb = part % C::kQBufs;
+        ok = ok && mbar_wait(&q_full[qb], (part / C::kQBufs) & 1, p.err);
+        for (int i = 0; i < n_tiles; ++i, ++it) {
+          // S(it): K-major codes, 32 dims a step
+          ok = ok && mbar_wait(&full[it % kStages], (it / kStages) & 1, p.err);
+          if (ok) {
+            tc_fence_after();
+            const uint32_t ak = tiles + (it % kStages) * kBStage, q = aq + qb * C::kQBytes;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8(tmem + 2 * kCols, sdesc(av + kk * 32 * 128, 16, 1024),
-                   sdesc_plain(pb + kk * 512, 128, 2048), id_o, o > 0 || kk > 0);
-          tc_commit(&o_done[o & 1]);
-          tc_commit(&empty[o % kStages]);
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f8(tmem + (it & 1) * kCols, sdesc(ak + kk * 32, 16, 1024),
+                     sdesc(q + kk * 32, 16, 1024), id_s, kk > 0);
+            tc_commit(&s_full[it & 1]);
+            if (i == n_tiles - 1) tc_commit(&q_empty[qb]);
+          }
+          if (it > 0) issue_o(it - 1, fresh);
+          fresh = i == 0;
         }
       }
+      __syncwarp();
+      ++part;
+      cur.advance();
+    }
+    if (lane == 0) {
+      issue_o(it - 1, fresh);
       if (!ok) {  // given up: let the products in flight finish before the memory goes
         tc_commit(drain);
         mbar_wait(drain, 0, nullptr);
       }
     }
+  } else if (warp >= 6) {
+    // -------------------------------- Q loaders --------------------------------
+    int part = 0;
+    bool ok = true;
+    while (cur.next(p, sq_info, n_tiles, lane)) {
+      const int qb = part % C::kQBufs;
+      if (part >= C::kQBufs)
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((part / C::kQBufs) & 1) ^ 1,
+                                                     p.err));
+      if (ok) {
+        load_q<T, HP>(p, sq_info.q0, kvh, sq_info.q_len * p.group, sq + qb * C::kQBytes,
+                      rowf + qb * HP, warp - 6, lane);
+        fence_async_smem();
+        mbar_arrive(&q_full[qb]);
+      }
+      ++part;
+      cur.advance();
+    }
   } else {
     // ------------------------------ compute warps ------------------------------
     const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
     const int key = threadIdx.x;  // this thread's key of a tile, and its dim of O
+    bool alive = true;
+    int it = 0, part = 0;
+    for (; cur.next(p, sq_info, n_tiles, lane); ++part, cur.advance()) {
+    const int qb = part % C::kQBufs;
+    const int rows = sq_info.q_len * p.group, k_len = sq_info.k_len;
+    const uint32_t q0 = sq_info.q0;
+    const float* rf = rowf + qb * HP;
     if (threadIdx.x < HP) {
       const int r = threadIdx.x;
-      rowlim[r] = r >= rows ? -1 : p.causal ? k_len - q_len + r / p.group : k_len - 1;
+      rowlim[r] = r >= rows ? -1 : p.causal ? k_len - sq_info.q_len + r / p.group : k_len - 1;
     }
-    load_q<T, HP>(p, q0, kvh, rows, sq, rowf, warp, lane);
-    fence_async_smem();
-    mbar_arrive(q_full);
-    bar_compute();  // rowf, rowlim
+    // a wait that runs out is not repeated, but the warp stays in step with the
+    // others' barriers to the end of the share
+    alive = alive && __all_sync(0xffffffffu,
+                                mbar_wait(&q_full[qb], (part / C::kQBufs) & 1, p.err));
+    bar_compute();  // rowlim
     float M[HP], l[HP];
 #pragma unroll
     for (int r = 0; r < HP; ++r) M[r] = -INFINITY, l[r] = 0.f;
-    bool alive = true;
-    for (int it = 0; it < ntiles; ++it) {
+    for (int i = 0; i < n_tiles; ++i, ++it) {
       const int s = it % kStages, x = it & 1;
-      // a wait that runs out is not repeated, but the warp stays in step with the
-      // others' barriers to the end of the loop
       alive = alive && __all_sync(0xffffffffu, mbar_wait(&full[s], (it / kStages) & 1, p.err) &&
                                                    mbar_wait(&s_full[x], (it >> 1) & 1, p.err));
       tc_fence_after();
@@ -395,7 +556,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       // log2 of the V scale, a power of two (a cleared pool's 0 counts as the least;
       // the upper bound keeps a stale block's NaN out of the masked sums)
       const int ev = min(max((int)(__float_as_uint(sc.y) >> 23 & 0xffu) - 127, -100), 120);
-      const int j = tok0 + it * kBTile + key;
+      const int j = (cur.t + i) * kBTile + key;
       float z[HP];
       const uint32_t cs = lane_addr + x * kCols;
       if constexpr (HP == 4) {
@@ -421,7 +582,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       float mine = -INFINITY;  // lane r: the warp's maximum of row r
 #pragma unroll
       for (int r = 0; r < HP; ++r) {
-        z[r] = j <= rowlim[r] ? z[r] * (rowf[r] * ks) + (float)ev : -INFINITY;
+        z[r] = j <= rowlim[r] ? z[r] * (rf[r] * ks) + (float)ev : -INFINITY;
         const float m = redux_max(z[r]);
         if (lane == r) mine = m;
       }
@@ -434,7 +595,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       for (int r = 0; r < HP; ++r) {
         const float m = fmaxf(fmaxf(rd[r], rd[HP + r]), fmaxf(rd[2 * HP + r], rd[3 * HP + r]));
         fac[r] = 1.f;
-        if (m > M[r]) {
+        if (m > M[r] + kHeadroom) {
           fac[r] = ex2_mufu(M[r] - m);
           M[r] = m;
           grew = true;
@@ -443,13 +604,13 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       if (grew) {
 #pragma unroll
         for (int r = 0; r < HP; ++r) l[r] *= fac[r];
-        if (it > 0) {  // O is in units of 2^M
+        if (i > 0) {  // O is in units of 2^M
           alive = alive && __all_sync(0xffffffffu,
                                       mbar_wait(&o_done[x ^ 1], ((it - 1) >> 1) & 1, p.err));
           tc_fence_after();
           constexpr int n = HP == 4 ? 4 : 8;
 #pragma unroll
-          for (int pc = 0; pc < 3; ++pc)
+          for (int pc = 0; pc < kPPieces; ++pc)
 #pragma unroll
             for (int c = 0; c < HP; c += n) {
               const uint32_t a = lane_addr + 2 * kCols + pc * HP + c;
@@ -474,11 +635,9 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
           tmem_wait_st();
         }
       }
-      // weights, times 256 for the pieces; the row sums without the V scale
+      // weights, scaled for the pieces; the row sums without the V scale
       const float unscale = __uint_as_float((uint32_t)(127 - ev) << 23);
-      uint32_t w[kCols / 4];
-#pragma unroll
-      for (int i = 0; i < kCols / 4; ++i) w[i] = 0u;
+      uint32_t w[C::kPCols / 4];
 #pragma unroll
       for (int c = 0; c < HP; c += 4) {
         float e[4];
@@ -487,22 +646,22 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
           const float m = M[c + r] == -INFINITY ? 0.f : M[c + r];
           e[r] = ex2_mufu(z[c + r] - m);
           l[c + r] += e[r] * unscale;
-          e[r] *= 256.f;
+          e[r] *= kWeight;
         }
-        uint32_t pw[3];
+        uint32_t pw[kPPieces];
         pieces4(e[0], e[1], e[2], e[3], pw);
 #pragma unroll
-        for (int pc = 0; pc < 3; ++pc) w[(pc * HP + c) / 4] = pw[pc];
+        for (int pc = 0; pc < kPPieces; ++pc) w[(pc * HP + c) / 4] = pw[pc];
       }
       if (it >= 2)  // this buffer's last reader
         alive = alive &&
                 __all_sync(0xffffffffu, mbar_wait(&o_done[x], ((it - 2) >> 1) & 1, p.err));
       uint8_t* dst = sp + x * C::kPBytes + key * 16;
 #pragma unroll
-      for (int nb = 0; nb < kCols / 16; ++nb)
+      for (int nb = 0; nb < C::kPCols / 16; ++nb)
         *reinterpret_cast<uint4*>(dst + nb * 2048) =
             make_uint4(w[4 * nb], w[4 * nb + 1], w[4 * nb + 2], w[4 * nb + 3]);
-      if (j >= tok1) {  // a key past the end: its V row may hold NaN codes, and 0 x NaN is NaN
+      if (j >= k_len) {  // a key past the end: its V row may hold NaN codes, and 0 x NaN is NaN
         uint8_t* vr = smem + s * kBStage + kBCode + key * 128;
 #pragma unroll
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vr + c * 16) = make_uint4(0, 0, 0, 0);
@@ -512,10 +671,11 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       mbar_arrive(&p_full[x]);
     }
 
+    mbar_arrive(&q_empty[qb]);  // this part's row factors have been read
+
     // ------------------------------- epilogue -------------------------------
-    if (alive && ntiles > 0)
-      alive = __all_sync(0xffffffffu, mbar_wait(&o_done[(ntiles - 1) & 1],
-                                                ((ntiles - 1) >> 1) & 1, p.err));
+    alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[(it - 1) & 1],
+                                                       ((it - 1) >> 1) & 1, p.err));
     tc_fence_after();
     bar_compute();  // the last tile's maxima have been read
 #pragma unroll
@@ -526,26 +686,29 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       if (lane == 0) red[warp * HP + r] = v;
     }
     bar_compute();
+    const bool whole = n_tiles == sq_info.tiles;
+    const int slot = 2 * cta + (cur.t == 0 ? 1 : 0);
+    if (!whole && key == 0)
+      p.ws_desc[slot] = make_int2(alive ? cur.b : -1, cur.t + n_tiles == sq_info.tiles);
     constexpr int n = HP == 4 ? 4 : 8;
     for (int c = 0; c < HP; c += n) {
-      float o[3][n];
+      float o[kPPieces][n];
 #pragma unroll
-      for (int pc = 0; pc < 3; ++pc) tmem_ldn<n>(lane_addr + 2 * kCols + pc * HP + c, o[pc]);
+      for (int pc = 0; pc < kPPieces; ++pc) tmem_ldn<n>(lane_addr + 2 * kCols + pc * HP + c, o[pc]);
       tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < n; ++i) {
         const int r = c + i;
         if (r >= rows || !alive) continue;
         const float ls = red[r] + red[HP + r] + red[2 * HP + r] + red[3 * HP + r];
-        const float acc = (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2) *
-                          (1.f / 256.f);
+        const float acc = (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2 +
+                           o[3][i] * kPiece3) * (1.f / kWeight);
         const float val = ls == 0.f ? 0.f : acc / ls;
-        if (nsplit == 1) {
+        if (whole) {
           const int64_t at = (int64_t)(q0 + r / p.group) * p.hq + kvh * p.group + r % p.group;
           static_cast<T*>(p.out)[at * kBD + key] = DT<T>::from_f(val);
         } else {
-          const int64_t at =
-              (((int64_t)b * p.max_splits + split) * p.hkv + kvh) * (p.q_cap * p.group) + r;
+          const int64_t at = (int64_t)slot * (p.q_cap * p.group) + r;
           p.ws_o[at * kBD + key] = val;
           float Mr = -INFINITY;
 #pragma unroll
@@ -553,6 +716,8 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
           if (key == 0) p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr + log2f(ls);
         }
       }
+    }
+    bar_compute();  // the sums have been read
     }
   }
 
@@ -565,31 +730,45 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
   }
 }
 
-// Joins the splits of one (sequence, row): weights 2^(lse - max lse).
+// Joins the parts of a sequence that the shares' cuts go through: block (cta, row)
+// starts from the CTA whose share holds the sequence's first part, follows the
+// next shares' first parts up to the last one, and weighs them by 2^(lse - max).
+// Lane i looks at the i-th part after the first; 32 parts a step.
 template <typename T>
 __global__ void __launch_bounds__(kBD) combine_fp8b_kernel(const Params p) {
   pdl_wait();
-  const int cap = p.q_cap * p.group;
-  const int kvh = blockIdx.x / cap, r = blockIdx.x % cap, b = blockIdx.y;
+  const int cta = blockIdx.x, r = blockIdx.y, kvh = cta % p.hkv, lane = threadIdx.x & 31;
+  const int ctas = p.groups * p.hkv, cap = p.q_cap * p.group;
+  const int b = p.ws_desc[2 * cta + 1].x;
+  if (b < 0) return;
   const uint32_t q0 = p.cu_q[b];
-  const int q_len = (int)(p.cu_q[b + 1] - q0);
-  const int k_len = (int)(p.cu_k[b + 1] - p.cu_k[b]);
-  const int nsplit = k_len > 0 ? (k_len + p.chunk - 1) / p.chunk : 1;
-  // the decode grid wrote no partials for these
-  if (nsplit <= 1 || q_len <= 0 || q_len > p.q_cap || r >= q_len * p.group || k_len > p.max_k ||
-      (int64_t)q0 + q_len > p.num_q_rows || (q_len > 1 && k_len < q_len))
-    return;
-  const int64_t step = (int64_t)p.hkv * cap;
-  const int64_t base = (int64_t)b * p.max_splits * step + (int64_t)kvh * cap + r;
-  float mx = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, p.ws_lse[base + s * step]);
-  const float mu = mx == -INFINITY ? 0.f : mx;
-  float wsum = 0.f, acc = 0.f;
+  if (r >= (int)(p.cu_q[b + 1] - q0) * p.group) return;
+  float mx = p.ws_lse[(int64_t)(2 * cta + 1) * cap + r], wsum = mx == -INFINITY ? 0.f : 1.f;
+  float acc = wsum * p.ws_o[((int64_t)(2 * cta + 1) * cap + r) * kBD + threadIdx.x];
+  for (int first = cta + p.hkv;; first += 32 * p.hkv) {
+    const int c = first + lane * p.hkv;
+    const int2 d = c < ctas ? p.ws_desc[2 * c] : make_int2(-1, 0);
+    const uint32_t mine = __ballot_sync(0xffffffffu, d.x == b);
+    const uint32_t last = __ballot_sync(0xffffffffu, d.x == b && d.y);
+    // parts of this step: up to the last one, or as far as they go without a gap
+    const int n = last ? __ffs(last) : min(32, __ffs(~mine) - 1 < 0 ? 32 : __ffs(~mine) - 1);
+    const float lse = lane < n ? p.ws_lse[(int64_t)(2 * c) * cap + r] : -INFINITY;
+    float m = lse;
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) m = warp_max_xor(m, x);
+    m = fmaxf(m, mx);
+    const float mu = m == -INFINITY ? 0.f : m;
+    const float old = exp2f(mx - mu), w = exp2f(lse - mu);
+    mx = m;
+    wsum *= old;
+    acc *= old;
 #pragma unroll 4
-  for (int s = 0; s < nsplit; ++s) {
-    const float w = exp2f(p.ws_lse[base + s * step] - mu);
-    wsum += w;
-    acc += w * p.ws_o[(base + s * step) * kBD + threadIdx.x];
+    for (int i = 0; i < n; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      wsum += wi;
+      acc += wi * p.ws_o[((int64_t)(2 * (first + i * p.hkv)) * cap + r) * kBD + threadIdx.x];
+    }
+    if (last || n < 32) break;
   }
   const int64_t at = (int64_t)(q0 + r / p.group) * p.hq + kvh * p.group + r % p.group;
   static_cast<T*>(p.out)[at * kBD + threadIdx.x] = DT<T>::from_f(wsum == 0.f ? 0.f : acc / wsum);
@@ -597,20 +776,22 @@ __global__ void __launch_bounds__(kBD) combine_fp8b_kernel(const Params p) {
 
 int padded_rows(int rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
-// Split plan: as many CTAs as ~3 resident waves, chunks of at least 6 tiles;
-// nothing is split when one CTA per (sequence, kv head) fills most of a wave and
-// no sequence is long.
-void plan(int num_seqs, int hkv, int max_k, int rows, int* chunk, int* max_splits) {
-  const int per_sm = padded_rows(rows) <= 8 ? 2 : 1;
-  const int tiles = max_k > 0 ? (max_k + kBTile - 1) / kBTile : 1;
-  const int64_t items = (int64_t)num_seqs * hkv, wave = 148 * per_sm;
-  int splits = (int)((3 * wave + items - 1) / items);
-  splits = std::min(splits, (tiles + 5) / 6);
-  if (items * 5 >= wave * 4 && tiles <= 24) splits = 1;
-  splits = std::max(splits, 1);
-  const int per = (tiles + splits - 1) / splits;
-  *chunk = per * kBTile;
-  *max_splits = (tiles + per - 1) / per;
+// Shares of the batch: one resident wave of CTAs, a share being Hkv of them.
+int shares(int hkv, int rows) {
+  return std::max(1, 148 * (padded_rows(rows) <= 8 ? 2 : 1) / hkv);
+}
+// Workspace: descriptors, log-sum-exps and partial rows of every CTA's two slots.
+struct Partials {
+  size_t lse, o, total;
+};
+Partials partials(int hq, int hkv, int q_cap) {
+  const size_t slots = 2 * (size_t)shares(hkv, q_cap * (hq / hkv)) * hkv;
+  const size_t rows = slots * q_cap * (hq / hkv);
+  Partials w;
+  w.lse = (slots * sizeof(int2) + 15) & ~size_t(15);
+  w.o = (w.lse + rows * sizeof(float) + 15) & ~size_t(15);
+  w.total = w.o + rows * kBD * sizeof(float);
+  return w;
 }
 
 template <typename T, int HP>
@@ -619,11 +800,11 @@ int launch(const AttnArgs& a, const Params& p, const CUtensorMap& mk, const CUte
   static unsigned long long done = 0;
   int rc = ensure_smem_attr((const void*)kern, Cfg<HP>::kSmem, &done);
   if (!rc)
-    rc = launch_pdl(kern, dim3(p.max_splits, a.hkv, a.num_seqs), dim3(kBThreads), Cfg<HP>::kSmem,
-                    a.stream, "decode fp8b launch", mk, mv, p);
-  if (!rc && p.max_splits > 1)
-    rc = launch_pdl(combine_fp8b_kernel<T>, dim3(a.hkv * p.q_cap * p.group, a.num_seqs),
-                    dim3(kBD), 0, a.stream, "combine fp8b launch", p);
+    rc = launch_pdl(kern, dim3(p.groups * a.hkv), dim3(kBThreads), Cfg<HP>::kSmem, a.stream,
+                    "decode fp8b launch", mk, mv, p);
+  if (!rc)
+    rc = launch_pdl(combine_fp8b_kernel<T>, dim3(p.groups * a.hkv, p.q_cap * p.group), dim3(kBD), 0,
+                    a.stream, "combine fp8b launch", p);
   return rc;
 }
 template <typename T>
@@ -639,13 +820,7 @@ int launch_rows(int rows, const AttnArgs& a, const Params& p, const CUtensorMap&
 
 }  // namespace
 
-size_t decode_fp8b_bytes(int num_seqs, int hq, int hkv, int max_k, int q_cap) {
-  int chunk, splits;
-  plan(num_seqs, hkv, max_k, q_cap * (hq / hkv), &chunk, &splits);
-  if (splits <= 1) return 0;
-  const size_t n = (size_t)num_seqs * splits * hq * q_cap;
-  return n * (kBD + 1) * sizeof(float);
-}
+size_t decode_fp8b_bytes(int hq, int hkv, int q_cap) { return partials(hq, hkv, q_cap).total; }
 
 int launch_decode_fp8b(const AttnArgs& a, int q_cap, bool all) {
   CUtensorMap mk, mv;
@@ -676,9 +851,13 @@ int launch_decode_fp8b(const AttnArgs& a, int q_cap, bool all) {
   p.causal = a.causal;
   p.scale_log2 = a.scale * kLog2e_;
   p.err = device_error_word();
-  plan(a.num_seqs, a.hkv, a.max_k, q_cap * p.group, &p.chunk, &p.max_splits);
-  p.ws_o = static_cast<float*>(a.ws);
-  p.ws_lse = p.ws_o + (size_t)a.num_seqs * p.max_splits * a.hq * q_cap * kBD;
+  p.num_seqs = a.num_seqs;
+  p.groups = shares(a.hkv, q_cap * p.group);
+  const Partials w = partials(a.hq, a.hkv, q_cap);
+  uint8_t* ws = static_cast<uint8_t*>(a.ws);
+  p.ws_desc = reinterpret_cast<int2*>(ws);
+  p.ws_lse = reinterpret_cast<float*>(ws + w.lse);
+  p.ws_o = reinterpret_cast<float*>(ws + w.o);
   return a.dtype == NVKV_DTYPE_BF16 ? launch_rows<__nv_bfloat16>(q_cap * p.group, a, p, mk, mv)
                                     : launch_rows<__half>(q_cap * p.group, a, p, mk, mv);
 }

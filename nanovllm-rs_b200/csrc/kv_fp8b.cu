@@ -171,7 +171,7 @@ Layout layout(int num_seqs, int hq, int hkv, int max_q, int max_k, int64_t promp
   Layout L = {0, 0, 0, 0, 0};
   if (num_seqs <= 0 || max_q <= 0) return L;
   const int cap = short_rows(hq, hkv, max_q);
-  L.base = decode_fp8b_bytes(num_seqs, hq, hkv, max_k, cap);
+  L.base = decode_fp8b_bytes(hq, hkv, cap);
   L.total = L.base;
   if (cap == max_q) return L;
   L.base = std::max(L.base, attention_workspace_bytes(num_seqs, hq, hkv, max_q, max_k));
