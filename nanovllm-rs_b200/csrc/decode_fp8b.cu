@@ -15,9 +15,10 @@
 // scores, multiplies by the key block's K scale, and forms z = S + log2(V
 // scale), so a weight 2^(z - M) already carries the value's scale and O needs
 // none; the row sum takes the scale back out (an exact power of two).  M is a
-// row's maximum of z over the CTA's keys, to within a headroom: warp maxima by
-// redux.sync, joined over the four warps through shared memory with one named
-// barrier a tile; when M moves the threads rescale O in TMEM.  Weights leave as one or
+// row's maximum of z over the CTA's keys, to within a headroom: one barrier with a
+// reduced flag a tile says whether any score has left it; only then are maxima
+// joined (redux.sync in a warp, shared memory over the four) and O rescaled in
+// TMEM.  Weights leave as one or
 // more 16-byte stores a thread (N-major B operand).
 //
 //   warps 0-3  compute (TMEM lanes 32 w .. 32 w + 31)
@@ -84,8 +85,8 @@ struct Cfg {
   static constexpr int kOffQ = kStages * kBStage;
   static constexpr int kOffP = kOffQ + kQBufs * kQBytes;
   static constexpr int kOffScale = kOffP + 2 * kPBytes;
-  static constexpr int kOffRed = kOffScale + kStages * kBScale * 4;  // [2][4][HP] maxima
-  static constexpr int kOffRow = kOffRed + 2 * 4 * HP * 4;           // [2][HP] factors, [HP] limits
+  static constexpr int kOffRed = kOffScale + kStages * kBScale * 4;  // [4][HP] maxima, sums
+  static constexpr int kOffRow = kOffRed + 4 * HP * 4;           // [2][HP] factors, [HP] limits
   static constexpr int kOffBar = kOffRow + 3 * HP * 4;
   static constexpr int kBars = 2 * kStages + 11;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
@@ -200,10 +201,37 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
+// A wait that has mostly ended already: one test (a try_wait may suspend the
+// thread, and took ~220 cycles even on a finished phase), then the bounded wait.
+__device__ __forceinline__ bool mbar_ready(uint64_t* bar, uint32_t parity, int* err) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, ok)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 __device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The compute warps' barrier, returning whether any thread's flag was set.
+__device__ __forceinline__ bool bar_compute_any(bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)flag)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ float redux_max(float x) {
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
@@ -532,7 +560,6 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     const int qb = part % C::kQBufs;
     const int rows = sq_info.q_len * p.group, k_len = sq_info.k_len;
     const uint32_t q0 = sq_info.q0;
-    const float* rf = rowf + qb * HP;
     if (threadIdx.x < HP) {
       const int r = threadIdx.x;
       rowlim[r] = r >= rows ? -1 : p.causal ? k_len - sq_info.q_len + r / p.group : k_len - 1;
@@ -542,13 +569,21 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     alive = alive && __all_sync(0xffffffffu,
                                 mbar_wait(&q_full[qb], (part / C::kQBufs) & 1, p.err));
     bar_compute();  // rowlim
+    // a row's factor and last visible key, in registers where there is room
+    constexpr bool kRegs = HP <= 8;
+    float rf_r[kRegs ? HP : 1];
+    int lim_r[kRegs ? HP : 1];
+    if constexpr (kRegs) {
+#pragma unroll
+      for (int r = 0; r < HP; ++r) rf_r[r] = rowf[qb * HP + r], lim_r[r] = rowlim[r];
+    }
     float M[HP], l[HP];
 #pragma unroll
     for (int r = 0; r < HP; ++r) M[r] = -INFINITY, l[r] = 0.f;
     for (int i = 0; i < n_tiles; ++i, ++it) {
       const int s = it % kStages, x = it & 1;
-      alive = alive && __all_sync(0xffffffffu, mbar_wait(&full[s], (it / kStages) & 1, p.err) &&
-                                                   mbar_wait(&s_full[x], (it >> 1) & 1, p.err));
+      alive = alive && mbar_ready(&s_full[x], (it >> 1) & 1, p.err) &&
+              mbar_ready(&full[s], (it / kStages) & 1, p.err);
       tc_fence_after();
       const float2 sc = *reinterpret_cast<const float2*>(ssc + s * kBScale +
                                                          key / NVKV_FP8B_BLOCK * 2);
@@ -579,34 +614,36 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
             z[c + r] = a0[r] + a1[r] * kPiece1 + a2[r] * kPiece2;
         }
       }
-      float mine = -INFINITY;  // lane r: the warp's maximum of row r
+      bool over = false;  // a score past its row's headroom
 #pragma unroll
       for (int r = 0; r < HP; ++r) {
-        z[r] = j <= rowlim[r] ? z[r] * (rf[r] * ks) + (float)ev : -INFINITY;
-        const float m = redux_max(z[r]);
-        if (lane == r) mine = m;
+        const float f = kRegs ? rf_r[kRegs ? r : 0] : rowf[qb * HP + r];
+        z[r] = j <= (kRegs ? lim_r[kRegs ? r : 0] : rowlim[r]) ? z[r] * (f * ks) + (float)ev
+                                                               : -INFINITY;
+        over |= z[r] > M[r] + kHeadroom;
       }
-      float* rd = red + x * 4 * HP;
-      if (lane < HP) rd[warp * HP + lane] = mine;
-      bar_compute();
-      float fac[HP];
-      bool grew = false;
+      if (bar_compute_any(over)) {
+        // new maxima: of the warp's keys, lane r keeping row r's, then of the four warps'
+        float mine = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < HP; ++r) {
-        const float m = fmaxf(fmaxf(rd[r], rd[HP + r]), fmaxf(rd[2 * HP + r], rd[3 * HP + r]));
-        fac[r] = 1.f;
-        if (m > M[r] + kHeadroom) {
-          fac[r] = ex2_mufu(M[r] - m);
-          M[r] = m;
-          grew = true;
+        for (int r = 0; r < HP; ++r) {
+          const float m = redux_max(z[r]);
+          if (lane == r) mine = m;
         }
-      }
-      if (grew) {
+        if (lane < HP) red[warp * HP + lane] = mine;
+        bar_compute();
+        float fac[HP];
 #pragma unroll
-        for (int r = 0; r < HP; ++r) l[r] *= fac[r];
+        for (int r = 0; r < HP; ++r) {
+          const float m = fmaxf(fmaxf(red[r], red[HP + r]), fmaxf(red[2 * HP + r], red[3 * HP + r]));
+          const bool up = m > M[r] + kHeadroom;
+          fac[r] = up ? ex2_mufu(M[r] - m) : 1.f;
+          M[r] = up ? m : M[r];
+          l[r] *= fac[r];
+        }
+        bar_compute();  // (the next exchange may be the next tile's)
         if (i > 0) {  // O is in units of 2^M
-          alive = alive && __all_sync(0xffffffffu,
-                                      mbar_wait(&o_done[x ^ 1], ((it - 1) >> 1) & 1, p.err));
+          alive = alive && mbar_ready(&o_done[x ^ 1], ((it - 1) >> 1) & 1, p.err);
           tc_fence_after();
           constexpr int n = HP == 4 ? 4 : 8;
 #pragma unroll
@@ -654,8 +691,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
         for (int pc = 0; pc < kPPieces; ++pc) w[(pc * HP + c) / 4] = pw[pc];
       }
       if (it >= 2)  // this buffer's last reader
-        alive = alive &&
-                __all_sync(0xffffffffu, mbar_wait(&o_done[x], ((it - 2) >> 1) & 1, p.err));
+        alive = alive && mbar_ready(&o_done[x], ((it - 2) >> 1) & 1, p.err);
       uint8_t* dst = sp + x * C::kPBytes + key * 16;
 #pragma unroll
       for (int nb = 0; nb < C::kPCols / 16; ++nb)
@@ -677,7 +713,6 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[(it - 1) & 1],
                                                        ((it - 1) >> 1) & 1, p.err));
     tc_fence_after();
-    bar_compute();  // the last tile's maxima have been read
 #pragma unroll
     for (int r = 0; r < HP; ++r) {
       float v = l[r];
