@@ -176,21 +176,27 @@ struct Cursor {
   }
 };
 
-__device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+// Shared-memory descriptors as two words: the low one holds the address (in 16
+// bytes, so moving on within shared memory is one 32-bit add) and LBO, the high
+// one SBO, the version bit and the layout (2: SWIZZLE_128B, 0: none).
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) {
+  return (saddr >> 4) | ((lbo >> 4) << 16);
+}
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo, uint32_t layout) {
+  return (sbo >> 4) | (1u << 14) | (layout << 29);
 }
 // kind::f8f6f4, e4m3 x e4m3, f32 accumulate, M = 128
 __host__ __device__ constexpr uint32_t idesc_f8(int n, uint32_t a_mn, uint32_t b_mn) {
   return (1u << 4) | (a_mn << 15) | (b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ void mma_f8(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                       uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
@@ -482,55 +488,62 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
         mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err);
   } else if (warp == 5) {
     // ------------------------------- MMA issuer -------------------------------
+    // The whole warp walks the loop, one lane issues: the loop is the critical path
+    // of a tile, so descriptors move by 32-bit adds and ring positions by compares.
     constexpr uint32_t id_s = idesc_f8(kCols, 0, 0), id_o = idesc_f8(C::kPCols, 1, 1);
-    const uint32_t tiles = smem_u32(smem), aq = smem_u32(sq), ap = smem_u32(sp);
+    constexpr uint32_t hi128 = desc_hi(1024, 2), hi_p = desc_hi(2048, 0);
+    const uint32_t k0 = desc_lo(smem_u32(smem), 16), v0 = k0 + (kBCode >> 4);
+    const uint32_t p0 = desc_lo(smem_u32(sp), 128);
+    uint32_t s_st = 0, s_ph = 0, o_st = 0;  // ring positions of the S and O products
     int it = 0, part = 0;
-    bool ok = true, fresh = false;  // fresh: tile it - 1 was its part's first
-    // O += V^T . P of tile o: 32 keys a step
-    auto issue_o = [&](int o, bool first) {
-      ok = ok && mbar_wait(&p_full[o & 1], (o >> 1) & 1, p.err);
+    bool ok = true;
+    uint32_t more = 0;  // 0: tile it - 1 was its part's first
+    // O += V^T . P of tile it - 1: 32 keys a step
+    auto issue_o = [&] {
+      const uint32_t x = (uint32_t)(it - 1) & 1u;
+      ok = ok && mbar_ready(&p_full[x], ((uint32_t)(it - 1) >> 1) & 1u, p.err);
       if (!ok) return;
       tc_fence_after();
-      const uint32_t av = tiles + (o % kStages) * kBStage + kBCode;
-      const uint32_t pb = ap + (o & 1) * C::kPBytes;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        mma_f8(tmem + 2 * kCols, sdesc(av + kk * 32 * 128, 16, 1024),
-               sdesc_plain(pb + kk * 512, 128, 2048), id_o, !first || kk > 0);
-      tc_commit(&o_done[o & 1]);
-      tc_commit(&empty[o % kStages]);
-    };
-    while (cur.next(p, sq_info, n_tiles, lane)) {
       if (lane == 0) {
-        const int qb = part % C::kQBufs;
-        ok = ok && mbar_wait(&q_full[qb], (part / C::kQBufs) & 1, p.err);
-        for (int i = 0; i < n_tiles; ++i, ++it) {
-          // S(it): K-major codes, 32 dims a step
-          ok = ok && mbar_wait(&full[it % kStages], (it / kStages) & 1, p.err);
-          if (ok) {
-            tc_fence_after();
-            const uint32_t ak = tiles + (it % kStages) * kBStage, q = aq + qb * C::kQBytes;
+        const uint32_t v = v0 + o_st * (kBStage >> 4), pb = p0 + x * (C::kPBytes >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_f8(tmem + (it & 1) * kCols, sdesc(ak + kk * 32, 16, 1024),
-                     sdesc(q + kk * 32, 16, 1024), id_s, kk > 0);
+        for (uint32_t kk = 0; kk < 4; ++kk)
+          mma_f8(tmem + 2 * kCols, v + kk * (32 * 128 >> 4), hi128, pb + kk * (512 >> 4), hi_p, id_o,
+                 kk > 0 ? 1u : more);
+        tc_commit(&o_done[x]);
+        tc_commit(&empty[o_st]);
+      }
+      __syncwarp();
+      o_st = o_st + 1 == kStages ? 0 : o_st + 1;
+    };
+    for (; cur.next(p, sq_info, n_tiles, lane); ++part, cur.advance()) {
+      const int qb = part % C::kQBufs;
+      const uint32_t q = desc_lo(smem_u32(sq + qb * C::kQBytes), 16);
+      ok = ok && mbar_ready(&q_full[qb], (part / C::kQBufs) & 1, p.err);
+      for (int i = 0; i < n_tiles; ++i, ++it) {
+        ok = ok && mbar_ready(&full[s_st], s_ph, p.err);
+        if (ok) {  // S(it): K-major codes, 32 dims a step
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t k = k0 + s_st * (kBStage >> 4);
+#pragma unroll
+            for (uint32_t kk = 0; kk < 4; ++kk)
+              mma_f8(tmem + (it & 1) * kCols, k + kk * 2, hi128, q + kk * 2, hi128, id_s, kk > 0);
             tc_commit(&s_full[it & 1]);
             if (i == n_tiles - 1) tc_commit(&q_empty[qb]);
           }
-          if (it > 0) issue_o(it - 1, fresh);
-          fresh = i == 0;
+          __syncwarp();
+          s_st = s_st + 1 == kStages ? 0 : s_st + 1;
+          s_ph ^= s_st == 0 ? 1u : 0u;
         }
+        if (it > 0) issue_o();
+        more = i > 0 ? 1u : 0u;
       }
-      __syncwarp();
-      ++part;
-      cur.advance();
     }
-    if (lane == 0) {
-      issue_o(it - 1, fresh);
-      if (!ok) {  // given up: let the products in flight finish before the memory goes
-        tc_commit(drain);
-        mbar_wait(drain, 0, nullptr);
-      }
+    issue_o();
+    if (lane == 0 && !ok) {  // given up: let the products in flight finish before the memory goes
+      tc_commit(drain);
+      mbar_wait(drain, 0, nullptr);
     }
   } else if (warp >= 6) {
     // -------------------------------- Q loaders --------------------------------
@@ -555,7 +568,8 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
     const int key = threadIdx.x;  // this thread's key of a tile, and its dim of O
     bool alive = true;
-    int it = 0, part = 0;
+    int it = 0, part = 0, st = 0;  // st, st_ph: ring position
+    uint32_t st_ph = 0;
     for (; cur.next(p, sq_info, n_tiles, lane); ++part, cur.advance()) {
     const int qb = part % C::kQBufs;
     const int rows = sq_info.q_len * p.group, k_len = sq_info.k_len;
@@ -581,9 +595,11 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
 #pragma unroll
     for (int r = 0; r < HP; ++r) M[r] = -INFINITY, l[r] = 0.f;
     for (int i = 0; i < n_tiles; ++i, ++it) {
-      const int s = it % kStages, x = it & 1;
+      const int s = st, x = it & 1;
       alive = alive && mbar_ready(&s_full[x], (it >> 1) & 1, p.err) &&
-              mbar_ready(&full[s], (it / kStages) & 1, p.err);
+              mbar_ready(&full[s], st_ph, p.err);
+      st = st + 1 == kStages ? 0 : st + 1;
+      st_ph ^= st == 0 ? 1u : 0u;
       tc_fence_after();
       const float2 sc = *reinterpret_cast<const float2*>(ssc + s * kBScale +
                                                          key / NVKV_FP8B_BLOCK * 2);
