@@ -77,13 +77,15 @@ struct Cfg {
   static constexpr int kPCols = kPPieces * HP;
   static constexpr int kCtasPerSm = HP <= 8 ? 2 : 1;
   static constexpr int kStages = HP <= 8 ? 3 : HP == 16 ? 6 : 5;
-  static constexpr int kQBufs = HP == 8 ? 1 : 2;
   static constexpr int kQBytes = kCols * 128;
+  // from the first Q buffer to the second: at 8 rows the 8 unused columns of the
+  // first may be the second's rows (their scores are never read), so that two CTAs fit
+  static constexpr int kQStride = HP == 8 ? 3 * HP * 128 : kQBytes;
   static constexpr int kPBytes = kPCols * 128;  // one of two buffers
   static constexpr int kUsed = 2 * kCols + kPCols;  // tensor-memory columns: two S, one O
   static constexpr int kTmem = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static constexpr int kOffQ = kStages * kBStage;
-  static constexpr int kOffP = kOffQ + kQBufs * kQBytes;
+  static constexpr int kOffP = (kOffQ + kQStride + kQBytes + 1023) / 1024 * 1024;
   static constexpr int kOffScale = kOffP + 2 * kPBytes;
   static constexpr int kOffRed = kOffScale + kStages * kBScale * 4;  // [4][HP] maxima, sums
   static constexpr int kOffRow = kOffRed + 4 * HP * 4;           // [2][HP] factors, [HP] limits
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     mbar_init(drain, 1);
     fence_mbar_init();
   }
-  for (int i = threadIdx.x; i < C::kQBufs * C::kQBytes / 16; i += kBThreads)  // the unused columns
+  for (int i = threadIdx.x; i < (C::kQStride + C::kQBytes) / 16; i += kBThreads)  // the unused columns
     *reinterpret_cast<uint4*>(sq + i * 16) = make_uint4(0, 0, 0, 0);
   pdl_wait();  // inputs may come from the kernel before this one
 
@@ -517,9 +519,9 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       o_st = o_st + 1 == kStages ? 0 : o_st + 1;
     };
     for (; cur.next(p, sq_info, n_tiles, lane); ++part, cur.advance()) {
-      const int qb = part % C::kQBufs;
-      const uint32_t q = desc_lo(smem_u32(sq + qb * C::kQBytes), 16);
-      ok = ok && mbar_ready(&q_full[qb], (part / C::kQBufs) & 1, p.err);
+      const int qb = part & 1;
+      const uint32_t q = desc_lo(smem_u32(sq + qb * C::kQStride), 16);
+      ok = ok && mbar_ready(&q_full[qb], (part >> 1) & 1, p.err);
       for (int i = 0; i < n_tiles; ++i, ++it) {
         ok = ok && mbar_ready(&full[s_st], s_ph, p.err);
         if (ok) {  // S(it): K-major codes, 32 dims a step
@@ -550,12 +552,12 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     int part = 0;
     bool ok = true;
     while (cur.next(p, sq_info, n_tiles, lane)) {
-      const int qb = part % C::kQBufs;
-      if (part >= C::kQBufs)
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((part / C::kQBufs) & 1) ^ 1,
+      const int qb = part & 1;
+      if (part >= 2)
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((part >> 1) & 1) ^ 1,
                                                      p.err));
       if (ok) {
-        load_q<T, HP>(p, sq_info.q0, kvh, sq_info.q_len * p.group, sq + qb * C::kQBytes,
+        load_q<T, HP>(p, sq_info.q0, kvh, sq_info.q_len * p.group, sq + qb * C::kQStride,
                       rowf + qb * HP, warp - 6, lane);
         fence_async_smem();
         mbar_arrive(&q_full[qb]);
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     int it = 0, part = 0, st = 0;  // st, st_ph: ring position
     uint32_t st_ph = 0;
     for (; cur.next(p, sq_info, n_tiles, lane); ++part, cur.advance()) {
-    const int qb = part % C::kQBufs;
+    const int qb = part & 1;
     const int rows = sq_info.q_len * p.group, k_len = sq_info.k_len;
     const uint32_t q0 = sq_info.q0;
     if (threadIdx.x < HP) {
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     // a wait that runs out is not repeated, but the warp stays in step with the
     // others' barriers to the end of the share
     alive = alive && __all_sync(0xffffffffu,
-                                mbar_wait(&q_full[qb], (part / C::kQBufs) & 1, p.err));
+                                mbar_wait(&q_full[qb], (part >> 1) & 1, p.err));
     bar_compute();  // rowlim
     // a row's factor and last visible key, in registers where there is room
     constexpr bool kRegs = HP <= 8;
