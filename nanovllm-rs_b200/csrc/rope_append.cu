@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kApThreads, kWide ? 3 : 2)
   float2* cs = reinterpret_cast<float2*>(
       smem + (kF8 ? (size_t)(p.window + kApBlock - 1) * p.half * sizeof(double2) : 0));
   __shared__ int64_t slot_s[kApTable + 1];  // slots of tokens w0 - 1 ..
-  __shared__ int lead_s[kApMaxWindow], len_s[kApMaxWindow], nrun_s, from_s, to_s;
+  __shared__ int lead_s[kApMaxWindow], len_s[kApMaxWindow], nrun_s, to_s;
   __shared__ float duo_s[kApWarps][2];
   const int64_t w0 = (int64_t)blockIdx.x * p.window;
   const int n = (int)min((int64_t)p.window, p.num_tokens - w0);
@@ -480,9 +480,19 @@ __global__ void __launch_bounds__(kApThreads, kWide ? 3 : 2)
   // tables: a thread keeps one pair, 4 tokens a step
   const int pr = tid % 64;
   const double fr = pr < p.half ? p.inv_freq[pr] : 0.0;
-  if (pr < p.half)
-    for (int t = tid / 64; t < n; t += kApThreads / 64)
-      cs[t * p.half + pr] = rope_cs(p.positions[w0 + t], fr, (float)p.a);
+  auto table = [&](int from, int to) {
+    if (pr >= p.half) return;
+    for (int t = from + tid / 64; t < to; t += kApThreads / 64) {
+      if constexpr (kF8) {
+        const double2 c = rope_cs64(p.positions[w0 + t], fr, p.a);
+        cs64[t * p.half + (pr & 3) * (p.half / 4) + (pr >> 2)] = c;
+        if (t < n) cs[t * p.half + pr] = make_float2((float)c.x, (float)c.y);
+      } else {
+        cs[t * p.half + pr] = rope_cs(p.positions[w0 + t], fr, (float)p.a);
+      }
+    }
+  };
+  table(0, n);
   if (warp == kApWarps - 1) {
     const int64_t t = w0 - 1 + lane;  // lane 0: the token before the window
     int64_t s = -1;
@@ -514,16 +524,12 @@ __global__ void __launch_bounds__(kApThreads, kWide ? 3 : 2)
       const int end = __shfl_sync(0xffffffffu, lane - 1 + len, last);
       if (lane == 0) {
         nrun_s = __popc(leads);
-        from_s = leads ? __ffs(leads) - 2 : 0;  // tokens that the runs span
-        to_s = leads ? end : 0;
+        to_s = leads ? end : 0;  // behind the last run's last token
       }
     }
   }
   __syncthreads();
-  if (kF8 && pr < p.half)
-    for (int t = from_s + tid / 64; t < to_s; t += kApThreads / 64)
-      cs64[t * p.half + (pr & 3) * (p.half / 4) + (pr >> 2)] =
-          rope_cs64(p.positions[w0 + t], fr, p.a);
+  if (kF8) table(n, to_s);  // the last run may go on behind the window
 
   // rows of single tokens: a warp per token when the window is wide, else a few
   // heads of the token
@@ -577,6 +583,9 @@ __global__ void __launch_bounds__(kApThreads, kWide ? 3 : 2)
       const double2* c64 = cs64 + t * p.half;
       if (kWide && u.len == kApBlock)
         unit<T, kM, kWide, true, kInter>(p, u, ks, vs, scale, block0, false, c64, d, duo_s, warp,
+                                         lane);
+      else if (!kWide && u.len <= 2)  // a decode step's: one row pair
+        unit<T, 1, kWide, false, kInter>(p, u, ks, vs, scale, block0, only_v, c64, d, duo_s, warp,
                                          lane);
       else
         unit<T, kM, kWide, false, kInter>(p, u, ks, vs, scale, block0, only_v, c64, d, duo_s, warp,
