@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(1024)
   __shared__ uint64_t warp_tot[32];
   __shared__ uint64_t carry;
   __shared__ uint32_t last_fit;
+  pdl_launch_dependents();  // (one CTA: a dependent grid may be scheduled beside it)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint64_t cap = (uint64_t)capacity;
   if (tid == 0) {

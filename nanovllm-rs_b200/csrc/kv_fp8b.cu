@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(256)
                                const uint32_t* __restrict__ block_tables, int64_t bt_stride,
                                int64_t num_blocks, int page, int hkv, int lanes,
                                T* __restrict__ kbuf, T* __restrict__ vbuf, int* err) {
+  pdl_wait();
   const int b = blockIdx.x;
   const uint32_t ks = cu_kd[b];
   const int len = (int)(cu_kd[b + 1] - ks);
@@ -322,13 +323,14 @@ extern "C" int nvkv_paged_attention_fp8b(
   a.dtype = dtype;
   a.stream = reinterpret_cast<cudaStream_t>(stream);
   a.k_scale = kv_scale;
-  rc = launch_decode_fp8b(a, cap, !prompts);
-  if (rc || !prompts) return rc;
-  // the others: dequantise their keys, then the contiguous prefill
+  if (!prompts) return launch_decode_fp8b(a, cap, true);
+  // single rows on the decode kernel; the others' keys are dequantised (their row
+  // offsets come first, beside the decode grid) for the contiguous prefill
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint32_t* cu_kd = reinterpret_cast<uint32_t*>(ws + L.cu_kd);
   rc = launch_prompt_rows(cu_seqlens_q, cu_seqlens_k, num_seqs, max_seqlen_k, prompt_kv_tokens,
                           cu_kd, a.stream);
+  if (!rc) rc = launch_decode_fp8b(a, cap, false);
   if (rc) return rc;
   const dim3 grid((unsigned)num_seqs,
                   (unsigned)std::min(65535, (max_seqlen_k - 1) / kDeqKeys + 1));
@@ -337,16 +339,17 @@ extern "C" int nvkv_paged_attention_fp8b(
   const auto* v8 = static_cast<const uint8_t*>(v_cache);
   int* err = device_error_word();
   if (dtype == NVKV_DTYPE_BF16)
-    dequant_prompt_fp8b_kernel<<<grid, 256, 0, a.stream>>>(
-        k8, v8, kv_scale, cu_kd, block_tables, block_table_stride, num_blocks, page_size,
-        num_kv_heads, lanes, reinterpret_cast<__nv_bfloat16*>(ws + L.kbuf),
-        reinterpret_cast<__nv_bfloat16*>(ws + L.vbuf), err);
+    rc = launch_pdl(dequant_prompt_fp8b_kernel<__nv_bfloat16>, grid, dim3(256), 0, a.stream,
+                    "fp8b dequant launch", k8, v8, kv_scale, (const uint32_t*)cu_kd, block_tables,
+                    block_table_stride, num_blocks, page_size, num_kv_heads, lanes,
+                    reinterpret_cast<__nv_bfloat16*>(ws + L.kbuf),
+                    reinterpret_cast<__nv_bfloat16*>(ws + L.vbuf), err);
   else
-    dequant_prompt_fp8b_kernel<<<grid, 256, 0, a.stream>>>(
-        k8, v8, kv_scale, cu_kd, block_tables, block_table_stride, num_blocks, page_size,
-        num_kv_heads, lanes, reinterpret_cast<__half*>(ws + L.kbuf),
-        reinterpret_cast<__half*>(ws + L.vbuf), err);
-  rc = check_cuda(cudaGetLastError(), "fp8b dequant launch");
+    rc = launch_pdl(dequant_prompt_fp8b_kernel<__half>, grid, dim3(256), 0, a.stream,
+                    "fp8b dequant launch", k8, v8, kv_scale, (const uint32_t*)cu_kd, block_tables,
+                    block_table_stride, num_blocks, page_size, num_kv_heads, lanes,
+                    reinterpret_cast<__half*>(ws + L.kbuf), reinterpret_cast<__half*>(ws + L.vbuf),
+                    err);
   if (rc) return rc;
   AttnArgs c = a;
   c.k_cache = ws + L.kbuf;
