@@ -118,8 +118,9 @@ class Engine:
         self.cuda_graphs = cuda_graphs and self._cuda
         self._graphs: Dict[tuple, tuple] = {}
         self._last_key = None
-        self.bt_g = torch.zeros(B * self._w, dtype=torch.int32, **pin)
-        self.d_bt_g = torch.zeros(B * self._w, dtype=torch.int32, device=dev)
+        wg = -(-(-(-max_model_len // 1024) * 1024) // block_size)  # pages of the last bucket
+        self.bt_g = torch.zeros(B * wg, dtype=torch.int32, **pin)
+        self.d_bt_g = torch.zeros(B * wg, dtype=torch.int32, device=dev)
         self.graph_steps = 0
 
     def close(self) -> None:
