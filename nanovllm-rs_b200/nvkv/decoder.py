@@ -32,7 +32,8 @@ from typing import List, Optional
 import torch
 import torch.distributed as dist
 
-from qwen3_config import QWEN3_0_6B, QWEN3_4B, QWEN3_8B, QWEN3_32B, Qwen3Config  # noqa: F401
+from qwen3_config import (QWEN3_0_6B, QWEN3_4B, QWEN3_8B, QWEN3_32B, Qwen3Config,  # noqa: F401
+                          RopeScaling)
 
 from . import ops
 
@@ -203,6 +204,14 @@ class Qwen3TP:
         self.k_scales: List[torch.Tensor] = []  # fp8 pool only: [Nb, Hkv, P] f32
         self.v_scales: List[torch.Tensor] = []
         self.kv_fp8 = False
+        self.kv_scales: List[torch.Tensor] = []  # block-scaled fp8 pool: [Nb, Hkv, P / 16, 2]
+        self.kv_fp8b = False
+        # rotary frequencies of the routes through nvkv_rope_append
+        sc = cfg.rope_scaling or RopeScaling("plain")
+        inv_freq, self.rope_factor = ops.rope_frequencies(
+            D, cfg.rope_theta, sc.kind, sc.factor, sc.original_max_position, sc.beta_fast,
+            sc.beta_slow, sc.low_freq_factor, sc.high_freq_factor, sc.attention_factor)
+        self.inv_freq = inv_freq.to(self.device)
         self._bufs = {}
         self.comm = None
         self._own_comm = False
@@ -222,18 +231,36 @@ class Qwen3TP:
 
     # ---- KV pool (model_runner.rs:286-303): per layer [Nb, P, Hkv/tp, D] ----
     def allocate_kv_cache(self, num_blocks: int, block_size: int = 256, fill_random: bool = False,
-                          seed: int = 1, kv_fp8: bool = False) -> None:
+                          seed: int = 1, kv_fp8: bool = False, kv_fp8b: bool = False) -> None:
         """kv_fp8: the optional e4m3 pool (codes [Nb, P, Hkv, D] uint8 + f32 row
         scales [Nb, Hkv, P], nvkv_store_kvcache_fp8 / nvkv_paged_attention_fp8)
-        instead of the model dtype.  fill_random fills the pool with random
-        rows (through the fp8 store for an fp8 pool)."""
+        instead of the model dtype.  kv_fp8b: the block-scaled e4m3 pool (codes
+        and power-of-two scales [Nb, Hkv, P / 16, 2], nvkv_rope_append /
+        nvkv_paged_attention_fp8b).  fill_random fills the pool with random
+        rows (through the store of an fp8 pool)."""
+        if kv_fp8 and (kv_fp8b or self.cfg.rope_scaling is not None):
+            raise ValueError("kv_fp8 goes with neither kv_fp8b nor rope_scaling")
+        self.kv_scales, self.kv_fp8b = [], kv_fp8b
         shape = (num_blocks, block_size, self.hkv, self.cfg.head_dim)
         self.k_caches, self.v_caches, self.k_scales, self.v_scales = [], [], [], []
         self.kv_fp8 = kv_fp8
         g = torch.Generator(device=self.device).manual_seed(seed * 7919 + self.rank)
-        slots = torch.arange(num_blocks * block_size, device=self.device) if kv_fp8 else None
+        slots = (torch.arange(num_blocks * block_size, device=self.device)
+                 if kv_fp8 or kv_fp8b else None)
         for _ in range(self.cfg.num_hidden_layers):
-            if kv_fp8:
+            if kv_fp8b:
+                k = torch.zeros(shape, device=self.device, dtype=torch.uint8)
+                v = torch.zeros_like(k)
+                sc = torch.zeros(num_blocks, self.hkv, block_size // 16, 2, device=self.device)
+                if fill_random:
+                    for lo in range(0, num_blocks, 64):  # bounded temporaries
+                        rows = slots[lo * block_size:min(lo + 64, num_blocks) * block_size]
+                        rk = torch.randn((rows.numel(),) + shape[2:], generator=g,
+                                         device=self.device, dtype=self.dtype)
+                        ops.rope_append(None, rk, torch.randn_like(rk), torch.zeros_like(rows),
+                                        self.inv_freq, k, v, rows, kv_scale=sc)
+                self.kv_scales.append(sc)
+            elif kv_fp8:
                 k = torch.zeros(shape, device=self.device, dtype=torch.uint8)
                 v = torch.zeros_like(k)
                 ks = torch.zeros(num_blocks, self.hkv, block_size, device=self.device)
@@ -260,10 +287,32 @@ class Qwen3TP:
     def _attend(self, li: int, qkv: torch.Tensor, st: "Step", q_buf, o_buf, ws) -> None:
         """One layer's attention hot path: the q/k-norm + RoPE prologue with the
         KV-cache store, then paged attention (qwen3.rs:128-145), over the
-        model-dtype pool (the store fused into the prologue) or the fp8 pool
-        (prologue, fp8 store, fp8 attention)."""
+        model-dtype pool (the store fused into the prologue), the fp8 pool
+        (prologue, fp8 store, fp8 attention) or the block-scaled fp8 pool (one
+        launch for norm, rotation and append).  With scaled frequencies the
+        model-dtype pool is filled by nvkv_rope_append too."""
         cfg, D, eps = self.cfg, self.cfg.head_dim, self.cfg.rms_norm_eps
         L = self.layers[li]
+        if self.kv_fp8b or cfg.rope_scaling is not None:
+            T, sc = qkv.size(0), self.kv_scales[li] if self.kv_fp8b else None
+            q, k, v = (x.view(T, -1, D) for x in
+                       qkv.split([self.hq * D, self.hkv * D, self.hkv * D], 1))
+            ops.rope_append(q, k, v, st.positions, self.inv_freq, self.k_caches[li],
+                            self.v_caches[li], st.slot_mapping, kv_scale=sc,
+                            attn_factor=self.rope_factor, q_norm_w=L["qn"], k_norm_w=L["kn"],
+                            eps=eps, q_out=q_buf)
+            if self.kv_fp8b:
+                ops.paged_attention_fp8b(q_buf, self.k_caches[li], self.v_caches[li], sc,
+                                         st.cu_seqlens_q, st.cu_seqlens_k, st.block_tables,
+                                         st.max_seqlen_q, st.max_seqlen_k, self.scale,
+                                         prompt_kv_tokens=st.prompt_kv_tokens, out=o_buf,
+                                         workspace=ws)
+            else:
+                ops.paged_attention(q_buf, self.k_caches[li], self.v_caches[li],
+                                    st.cu_seqlens_q, st.cu_seqlens_k, st.block_tables,
+                                    st.max_seqlen_q, st.max_seqlen_k, self.scale, out=o_buf,
+                                    workspace=ws)
+            return
         if not self.kv_fp8:
             ops.qknorm_rope(qkv, st.positions, self.hq, self.hkv, L["qn"], L["kn"], eps,
                             cfg.rope_theta, cfg.max_position_embeddings, D,
@@ -286,7 +335,10 @@ class Qwen3TP:
 
     def _ws(self, st: "Step") -> torch.Tensor:
         B = st.cu_seqlens_q.numel() - 1
-        if self.kv_fp8:
+        if self.kv_fp8b:
+            n = ops.workspace_size_fp8b(B, self.hq, self.hkv, st.max_seqlen_q, st.max_seqlen_k,
+                                        st.prompt_kv_tokens, self.cfg.head_dim)
+        elif self.kv_fp8:
             n = ops.workspace_size_fp8(B, self.hq, self.hkv, st.max_seqlen_q, st.max_seqlen_k,
                                        st.prompt_kv_tokens, self.cfg.head_dim)
         else:
@@ -422,6 +474,9 @@ class Qwen3TP:
         embedding's fused call, the final norm being fused into the last
         layer's)."""
         B = st.cu_seqlens_q.numel() - 1
+        if self.kv_fp8b:  # norms, SiLU, append, decode, join; prompts: + offsets, keys, plan, prefill
+            short = st.max_seqlen_q * (self.hq // self.hkv) <= 32
+            return (6 + (0 if short else 4)) * self.cfg.num_hidden_layers + 1
         split = ops.workspace_size(B, self.hq, self.hkv, 1, st.max_seqlen_k) > 0
         per = 5 + (1 if split else 0) + (2 if st.max_seqlen_q > 1 else 0)
         if self.kv_fp8:  # + the fp8 store; prompts: + row offsets and dequantisation

@@ -7,6 +7,23 @@ libnvkv.so.  nvkv.decoder re-exports them.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How rotary frequencies are scaled for contexts past those of training
+    (nvkv.rope_frequencies): kind "plain", "linear", "ntk", "yarn" or "bands".
+    The reference has plain frequencies only (rotary_embedding.rs:28-57)."""
+
+    kind: str
+    factor: float = 1.0
+    original_max_position: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    attention_factor: float = 0.0  # 0: the kind's own
 
 
 @dataclass(frozen=True)
@@ -24,6 +41,7 @@ class Qwen3Config:
     rope_theta: float = 1e6
     max_position_embeddings: int = 40960
     tie_word_embeddings: bool = False
+    rope_scaling: Optional[RopeScaling] = None  # None: the reference's rotation
 
 
 QWEN3_0_6B = Qwen3Config(1024, 28, 16, 8, 3072, tie_word_embeddings=True)
