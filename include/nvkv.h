@@ -311,10 +311,11 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  *   lay them out; a token whose slot does not ascend from its neighbour's in
  *   the same block is not stored, nor those after it in that block, and
  *   NVKV_DEVERR_SLOT_ORDER is recorded.  A block that a call reaches again
- *   after other blocks ends up with unspecified contents (no other block
- *   does).
+ *   after other blocks or skipped tokens ends up with unspecified contents
+ *   (no other block does).
  * q/k/v: [T, H, 128] with token strides (elements, multiples of 4), rows
- * 8-byte aligned; num_q_heads may be 0 (q, q_out NULL).  q_out may be q.
+ * 8-byte aligned; num_q_heads may be 0 (q, q_out NULL).  q_out may be q; any
+ * other overlap of q_out, the inputs and the caches is refused.
  *
  * nvkv_load_kvcache_fp8b: k_out / v_out [n, Hkv, 128] = dtype(code * scale) of
  * rows slots[i] (negative: zeros; past the pool: zeros, recorded).  f16
@@ -327,7 +328,8 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * the others are dequantised into the workspace for the prefill kernel, so
  * the caller passes prompt_kv_tokens >= the sum of their k_len (a prompt that
  * does not fit is skipped and recorded as NVKV_DEVERR_SEQLEN).  Malformed
- * sequences are skipped and recorded as in nvkv_paged_attention.  Products
+ * sequences are skipped and recorded as in nvkv_paged_attention.  max_seqlen_k
+ * up to 2^30; out may be q when its rows are dense.  Products
  * are exact in the codes: queries enter as three e4m3 pieces (12 significant
  * bits), the softmax weights as four (2^-12 of a weight down to 2^-17 of the
  * row's largest), sums in f32.  Calls

@@ -12,6 +12,13 @@ Cases (one JSON line each; bytes/flops are the algorithmic figures):
   decode_8b_tp1   one layer of the Qwen3-8B TP1 decode step (B=256, 32q/8kv) (HBM)
   decode_8b_tp8   the same layer at TP8 per GPU (4q/1kv)                   (HBM)
   decode_32b_tp8  Qwen3-32B TP8 per GPU: B=64, 8q/1kv, L=32768            (HBM)
+  decode_*_fp8b   the same decode layers over the block-scaled pool
+                  (nvkv_paged_attention_fp8b)                            (HBM)
+  verify_8b_tp1_fp8b  64 sequences x 4 new tokens over that pool         (HBM)
+  rope_prefill    nvkv_rope, 16384 tokens, 32q/8kv heads                 (HBM)
+  append_fp8b_*   nvkv_rope_append into the block-scaled pool, a 256-token
+                  decode step and 16 prompts x 1024                      (HBM)
+  load_fp8b       nvkv_load_kvcache_fp8b, 16384 rows, 8 kv heads         (HBM)
   prefill_8b      tcgen05 prefill, Qwen3-8B TP1: 16 prompts x 1024, causal (tensor)
   step_metadata   device-side decode-step metadata, 256 sequences (latency)
   mixed_4b_tp1/2  config 3 (Qwen3-4B): 120 decodes + 8 fresh prompts in one
@@ -185,6 +192,95 @@ def case_decode_fp8(name, lens, hq, hkv, nblocks, iters, copies=1):
               8 * (B + 1))
     return dict(kernel=name, B=B, hq=hq, hkv=hkv, L_mean=float(np.mean(lens)), bytes=nbytes, s=med,
                 bound="hbm", kv="e4m3 + f32 row scales")
+
+
+def _fp8b_pool(nblocks, page, hkv):
+    k8 = torch.zeros(nblocks, page, hkv, 128, dtype=torch.uint8, device="cuda")
+    return k8, torch.zeros_like(k8), torch.zeros(nblocks, hkv, page // 16, 2, device="cuda")
+
+
+def case_decode_fp8b(name, lens, hq, hkv, nblocks, iters, copies=1, new=1):
+    """case_decode over the block-scaled pool, `new` query rows a sequence: codes
+    and scales written by nvkv_rope_append from random rows.  Algorithmic bytes:
+    one byte per K/V value, 4-byte scales per 16 slots, q and out, block tables."""
+    copies = COPIES or copies
+    page = 256
+    caches, bt = _paged(lens, page, hkv, nblocks, 3, copies)
+    freq, _ = ops.rope_frequencies(128, 1e6)
+    freq = freq.cuda()
+    slots = torch.arange(nblocks * page, device="cuda")
+    pools = []
+    for kc, vc in caches:
+        pools.append(_fp8b_pool(nblocks, page, hkv))
+        ops.rope_append(None, kc.view(-1, hkv, 128), vc.view(-1, hkv, 128), slots % 4096, freq,
+                        pools[-1][0], pools[-1][1], slots, kv_scale=pools[-1][2])
+    del caches
+    torch.cuda.empty_cache()
+    B = len(lens)
+    q = torch.randn(B * new, hq, 128, device="cuda").bfloat16()
+    cu_q = torch.arange(B + 1, dtype=torch.int32, device="cuda") * new
+    cu_k = torch.from_numpy(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)).cuda()
+    out = torch.empty_like(q)
+    ws = torch.empty(max(16, ops.workspace_size_fp8b(B, hq, hkv, new, int(max(lens)))),
+                     dtype=torch.uint8, device="cuda")
+    fn = lambda i: ops.paged_attention_fp8b(q, *pools[i % copies], cu_q, cu_k, bt, new,  # noqa
+                                            int(max(lens)), 128 ** -0.5, out=out, workspace=ws)
+    med, _ = _time(fn, iters)
+    nblk = sum((int(L) + page - 1) // page for L in lens)
+    blocks16 = sum((int(L) + 15) // 16 for L in lens)
+    nbytes = (int(np.sum(lens)) * hkv * 128 * 2 + blocks16 * hkv * 8 + 2 * B * new * hq * 128 * 2 +
+              4 * nblk + 8 * (B + 1))
+    return dict(kernel=name, B=B, hq=hq, hkv=hkv, L_mean=float(np.mean(lens)), bytes=nbytes, s=med,
+                bound="hbm", kv="e4m3, one f32 scale per 16 slots")
+
+
+def case_rope(T, iters):
+    hq, hkv = 32, 8
+    freq, _ = ops.rope_frequencies(128, 1e6)
+    freq = freq.cuda()
+    src = [(torch.randn(T, hq, 128, device="cuda").bfloat16(),
+            torch.randn(T, hkv, 128, device="cuda").bfloat16()) for _ in range(2)]
+    pos = torch.randint(0, 40960, (T,), device="cuda")
+    qo, ko = torch.empty_like(src[0][0]), torch.empty_like(src[0][1])
+    fn = lambda i: ops.rope(*src[i % 2], pos, freq, q_out=qo, k_out=ko)  # noqa
+    med, _ = _time(fn, iters)
+    return dict(kernel="rope", T=T, bytes=2 * T * (hq + hkv) * 128 * 2 + 8 * T, s=med, bound="hbm")
+
+
+def case_append_fp8b(seqs, new, iters, hq=32, hkv=8, page=256):
+    """`new` tokens for each of `seqs` sequences that start on a page: rotation of
+    q and K, the codes and scales, q out.  A decode step (new = 1) adds its row
+    at slot 9 of a block and so reads the nine before it."""
+    T = seqs * new
+    at = 9 if new == 1 else 0
+    pages = (at + new + page - 1) // page
+    pool = _fp8b_pool(seqs * pages, page, hkv)
+    freq, _ = ops.rope_frequencies(128, 1e6)
+    freq = freq.cuda()
+    slots = torch.cat([b * pages * page + at + torch.arange(new) for b in range(seqs)]).cuda()
+    copies = 8 if T < 4096 else 2
+    src = [[torch.randn(T, h, 128, device="cuda").bfloat16() for h in (hq, hkv, hkv)]
+           for _ in range(copies)]
+    pos = torch.randint(0, 40960, (T,), device="cuda")
+    qo = torch.empty_like(src[0][0])
+    fn = lambda i: ops.rope_append(*src[i % copies], pos, freq, pool[0], pool[1], slots,  # noqa
+                                   kv_scale=pool[2], q_out=qo)
+    med, _ = _time(fn, iters)
+    kept = seqs * at * hkv * 128 * 2
+    nbytes = (T * (hq + 2 * hkv) * 128 * 2 + T * hq * 128 * 2 + T * hkv * 128 * 2 + 16 * T + kept +
+              seqs * ((new + 15) // 16) * hkv * 8 * (2 if new == 1 else 1))
+    return dict(kernel="rope_append fp8b", T=T, bytes=nbytes, s=med, bound="hbm")
+
+
+def case_load_fp8b(T, iters, hkv=8, page=256):
+    pool = _fp8b_pool(T // page, page, hkv)
+    slots = torch.randperm(T, device="cuda")
+    outs = [torch.empty(T, hkv, 128, device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    fn = lambda i: ops.load_kvcache_fp8b(*pool, slots, torch.bfloat16, k_out=outs[i % 2],  # noqa
+                                         v_out=outs[2 + i % 2])
+    med, _ = _time(fn, iters)
+    return dict(kernel="load_kvcache_fp8b", T=T, bytes=T * hkv * 128 * 6 + T // 16 * hkv * 8 + 8 * T,
+                s=med, bound="hbm")
 
 
 def case_sample(name, B, V, iters):
@@ -452,6 +548,23 @@ CASES = {
         8),
     "decode_32b_tp8_fp8": lambda it: case_decode_fp8(
         "decode_32b_tp8_fp8", np.full(64, 32768), 8, 1, 64 * 128 + 2, it, 2),
+    "decode_8b_tp1_fp8b": lambda it: case_decode_fp8b(
+        "decode_8b_tp1_fp8b", np.random.default_rng(4).integers(1025, 1537, 256), 32, 8, 1560, it,
+        2),
+    "decode_8b_tp2_fp8b": lambda it: case_decode_fp8b(
+        "decode_8b_tp2_fp8b", np.random.default_rng(4).integers(1025, 1537, 256), 16, 4, 1560, it,
+        4),
+    "decode_8b_tp8_fp8b": lambda it: case_decode_fp8b(
+        "decode_8b_tp8_fp8b", np.random.default_rng(4).integers(1025, 1537, 256), 4, 1, 1560, it,
+        8),
+    "decode_32b_tp8_fp8b": lambda it: case_decode_fp8b(
+        "decode_32b_tp8_fp8b", np.full(64, 32768), 8, 1, 64 * 128 + 2, it, 2),
+    "verify_8b_tp1_fp8b": lambda it: case_decode_fp8b(
+        "verify_8b_tp1_fp8b", np.full(64, 2000), 32, 8, 64 * 8, it, 2, new=4),
+    "rope_prefill": lambda it: case_rope(16384, it),
+    "append_fp8b_decode": lambda it: case_append_fp8b(256, 1, it),
+    "append_fp8b_prefill": lambda it: case_append_fp8b(16, 1024, it),
+    "load_fp8b": lambda it: case_load_fp8b(16384, it),
     "sample_8b_tp1": lambda it: case_sample("sample_8b_tp1", 256, 151936, it),
     "sample_8b_tp8": lambda it: case_sample("sample_8b_tp8", 256, 151936 // 8, it),
     "decode_g16": lambda it: case_decode(

@@ -67,6 +67,11 @@ int encode_kv_tensor_map_u8(CUtensorMap* map, const void* base, int64_t row_byte
 bool rows_clash(const void* a, int64_t a_stride, int64_t a_row, const void* b, int64_t b_stride,
                 int64_t b_row, int64_t tokens);
 
+inline bool spans_meet(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Raises a kernel's dynamic shared-memory limit once per device (first call

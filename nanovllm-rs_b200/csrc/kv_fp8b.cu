@@ -276,8 +276,9 @@ extern "C" int nvkv_paged_attention_fp8b(
   if (block_table_stride < ((int64_t)max_seqlen_k + page_size - 1) / page_size)
     return set_error(NVKV_ERR_INVALID_ARG,
                      "paged_attention_fp8b: block_table_stride < blocks needed by max_seqlen_k");
-  if (num_blocks > 0x7fffffffLL / page_size)
-    return set_error(NVKV_ERR_UNSUPPORTED, "paged_attention_fp8b: more than 2^31 cache rows");
+  if (num_blocks > 0x7fffffffLL / page_size || max_seqlen_k > 1 << 30)
+    return set_error(NVKV_ERR_UNSUPPORTED,
+                     "paged_attention_fp8b: more than 2^31 cache rows or 2^30 keys a sequence");
   if (q_stride < (int64_t)num_q_heads * head_dim || q_stride % 8 != 0 || !aligned16(q) ||
       !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(kv_scale))
     return set_error(NVKV_ERR_ALIGNMENT, "paged_attention_fp8b: misaligned buffer or stride");
@@ -285,6 +286,9 @@ extern "C" int nvkv_paged_attention_fp8b(
     return set_error(NVKV_ERR_ALIGNMENT, "paged_attention_fp8b: metadata must be 4-byte aligned");
   if (!(softmax_scale > 0.f) || softmax_scale > 3e38f)
     return set_error(NVKV_ERR_INVALID_ARG, "paged_attention_fp8b: softmax_scale must be > 0");
+  const int64_t q_row = (int64_t)num_q_heads * head_dim;
+  if (rows_clash(q, q_stride, q_row, out, q_row, q_row, num_q_tokens))
+    return set_error(NVKV_ERR_INVALID_ARG, "paged_attention_fp8b: out overlaps q without being it");
   const int cap = short_rows(num_q_heads, num_kv_heads, max_seqlen_q);
   const bool prompts = cap < max_seqlen_q;
   if (prompts && prompt_kv_tokens == 0)

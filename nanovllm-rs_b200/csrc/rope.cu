@@ -276,7 +276,9 @@ extern "C" int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t
   // One wave of CTAs: a CTA costs two dependent loads, the table and a barrier
   // before it streams (the same 16384 tokens with four in flight: windows of 1 / 2
   // / 4 / 8 tokens 237 / 140 / 93 / 75 us).
-  p.window = (int)std::min<int64_t>(kRopeMaxWindow, (num_tokens + kRopeWave - 1) / kRopeWave);
+  // (the table of a window stays below the 48 KB that need no opt-in)
+  p.window = (int)std::min<int64_t>(std::min(kRopeMaxWindow, 48 * 1024 / (p.half * 8)),
+                                    (num_tokens + kRopeWave - 1) / kRopeWave);
   const int bx = std::min(p.units, 64);
   const int rounds = (p.heads * bx + 383) / 384;
   const int by = (p.heads + rounds - 1) / rounds;  // bx * by < 384 + bx

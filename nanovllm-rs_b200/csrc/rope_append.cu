@@ -655,6 +655,16 @@ extern "C" int nvkv_rope_append(const void* q, int64_t q_stride, const void* k, 
                 rows_clash(k, k_stride, kr, q_out, qr, qr, num_tokens) ||
                 rows_clash(v, v_stride, kr, q_out, qr, qr, num_tokens)))
     return set_error(NVKV_ERR_INVALID_ARG, "rope_append: q_out overlaps an input without being q");
+  const uint64_t pool = (uint64_t)num_blocks * page_size * kr * (kv_scale ? 1 : 2);
+  const uint64_t k_bytes = (uint64_t)((num_tokens - 1) * k_stride + kr) * 2;
+  const uint64_t v_bytes = (uint64_t)((num_tokens - 1) * v_stride + kr) * 2;
+  const uint64_t q_bytes = q ? (uint64_t)((num_tokens - 1) * q_stride + qr) * 2 : 0;
+  for (const void* c : {(const void*)k_cache, (const void*)v_cache})
+    if (spans_meet(c, pool, k, k_bytes) || spans_meet(c, pool, v, v_bytes) ||
+        spans_meet(c, pool, q, q_bytes) || spans_meet(c, pool, q_out, num_tokens * qr * 2))
+      return set_error(NVKV_ERR_INVALID_ARG, "rope_append: an input or q_out overlaps a cache");
+  if (spans_meet(k_cache, pool, v_cache, pool))
+    return set_error(NVKV_ERR_INVALID_ARG, "rope_append: k_cache and v_cache overlap");
   AppendParams p;
   p.q = q;
   p.k = k;

@@ -325,8 +325,8 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
         raise _bad("k_out without k")
     stream = _raw_stream(q, k, q_out, k_out, positions, inv_freq)
     check(lib.nvkv_rope(q.data_ptr(), qs, _at(k), ks, q_out.data_ptr(), qos, _at(k_out), kos, T,
-                        hq, hkv, d, positions.data_ptr(), inv_freq.data_ptr(), rot, attn_factor,
-                        1 if interleaved else 0, _dtype(q), stream))
+                        hq, hkv, d, positions.data_ptr(), inv_freq.data_ptr(), rot,
+                        float(attn_factor), 1 if interleaved else 0, _dtype(q), stream))
     return q_out, k_out
 
 
@@ -394,9 +394,9 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                          slot_mapping, q_norm_w, k_norm_w)
     check(lib.nvkv_rope_append(
         _at(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, T, hq, hkv, d, positions.data_ptr(),
-        inv_freq.data_ptr(), rot, attn_factor, 1 if interleaved else 0, _at(q_norm_w),
-        _at(k_norm_w), eps, _at(q_out), k_cache.data_ptr(), v_cache.data_ptr(), _at(kv_scale),
-        slot_mapping.data_ptr(), nb, page, _dtype(k), stream))
+        inv_freq.data_ptr(), rot, float(attn_factor), 1 if interleaved else 0, _at(q_norm_w),
+        _at(k_norm_w), float(eps), _at(q_out), k_cache.data_ptr(), v_cache.data_ptr(),
+        _at(kv_scale), slot_mapping.data_ptr(), nb, page, _dtype(k), stream))
     return q_out
 
 
@@ -450,6 +450,8 @@ def paged_attention_fp8b(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     needed when max_seqlen_q * Hq / Hkv > 32."""
     dt = q.dtype
     qs = _rows(q, dt)
+    max_seqlen_q, max_seqlen_k = int(max_seqlen_q), int(max_seqlen_k)
+    prompt_kv_tokens = int(prompt_kv_tokens)
     T, hq, d = q.shape
     nb, page, hkv, cd = _fp8b_pool(k_cache, v_cache, kv_scale)
     B = cu_seqlens_q.numel() - 1
@@ -475,7 +477,8 @@ def paged_attention_fp8b(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     check(lib.nvkv_paged_attention_fp8b(
         q.data_ptr(), qs, T, k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(), nb,
         out.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
-        block_tables.size(1), B, max_seqlen_q, max_seqlen_k, hq, hkv, d, page, softmax_scale,
+        block_tables.size(1), B, max_seqlen_q, max_seqlen_k, hq, hkv, d, page,
+        float(softmax_scale),
         1 if causal else 0, prompt_kv_tokens, _at(workspace), ws_bytes, _dtype(q), stream))
     return out
 

@@ -257,3 +257,65 @@ def test_append_then_attend_steps():
                         SHORT if max(new) <= 8 else prompt_err(q.dtype))
         have = k_lens
     assert nvkv.device_error() == 0
+
+
+def test_many_kv_heads_and_many_sequences():
+    """More kv heads than a wave has CTAs; more sequences than a CTA has threads,
+    empty ones among them (q_len 0: padding of a batch)."""
+    k_lens = [70, 3]
+    pool, bt, rows = filled(k_lens, 301, P=128, seed=21)
+    q = _q(2, 301, torch.bfloat16, 8)
+    out = _run(q, pool, bt, [1, 1], k_lens)
+    assert nvkv.device_error() == 0
+    check_attention(out, q, rows, [1, 1], k_lens, D ** -0.5, SHORT)
+    rng = np.random.default_rng(6)
+    k_lens = rng.integers(1, 200, 700).tolist()
+    q_lens = (rng.random(700) < 0.8).astype(int).tolist()
+    pool, bt, rows = filled(k_lens, 2, P=128, seed=22)
+    q = _q(sum(q_lens) + 3, 6, torch.float16, 9)  # three rows behind the last sequence
+    out = torch.full_like(q, 7.0)
+    nvkv.paged_attention_fp8b(q, *pool, cu(q_lens), cu(k_lens), bt, 1, 199, D ** -0.5, out=out)
+    torch.cuda.synchronize()
+    assert nvkv.device_error() == 0 and bool((out[-3:] == 7).all())
+    check_attention(out, q, rows, q_lens, k_lens, D ** -0.5, SHORT, every=7)
+
+
+def test_prompt_that_does_not_fit_is_reported():
+    """prompt_kv_tokens below the prompts' keys: that prompt's rows stay as they
+    were, the others are right."""
+    q_lens, k_lens = [300, 1, 200], [300, 900, 450]
+    pool, bt, rows = filled(k_lens, 2, seed=23)
+    q = _q(sum(q_lens), 4, torch.bfloat16, 3)
+    out = torch.full_like(q, 7.0)
+    nvkv.device_error()
+    nvkv.paged_attention_fp8b(q, *pool, cu(q_lens), cu(k_lens), bt, 300, 900, D ** -0.5,
+                              prompt_kv_tokens=500, out=out)
+    torch.cuda.synchronize()
+    assert nvkv.device_error() == DEVERR_SEQLEN and bool((out[301:] == 7).all())
+    check_attention(out[:300], q[:300], rows[:1], [300], [300], D ** -0.5, prompt_err(q.dtype))
+    check_attention(out[300:301], q[300:301], rows[1:2], [1], [900], D ** -0.5, SHORT)
+
+
+def test_two_streams_at_once_and_in_place():
+    """Calls that overlap on the GPU, each with its own workspace, and out = q:
+    the bits of a call alone."""
+    cases = []
+    for seed, k_lens in ((31, [4000, 100, 9]), (32, [700] * 40)):
+        pool, bt, _ = filled(k_lens, 2, seed=seed)
+        q = _q(len(k_lens), 8, torch.bfloat16, seed)
+        want = _run(q, pool, bt, [1] * len(k_lens), k_lens)
+        ws = torch.empty(nvkv.workspace_size_fp8b(len(k_lens), 8, 2, 1, max(k_lens)),
+                         device="cuda", dtype=torch.uint8)
+        cases.append((q, pool, bt, cu([1] * len(k_lens)), cu(k_lens), max(k_lens), want, ws,
+                      torch.cuda.Stream(), torch.empty_like(q)))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for q, pool, bt, cq, ck, mk, _, ws, stream, out in cases:
+            with torch.cuda.stream(stream):
+                nvkv.paged_attention_fp8b(q, *pool, cq, ck, bt, 1, mk, D ** -0.5, out=out,
+                                          workspace=ws)
+    torch.cuda.synchronize()
+    for q, pool, bt, cq, ck, mk, want, ws, _, out in cases:
+        assert torch.equal(out, want)
+        nvkv.paged_attention_fp8b(q, *pool, cq, ck, bt, 1, mk, D ** -0.5, out=q, workspace=ws)
+        assert torch.equal(q, want)

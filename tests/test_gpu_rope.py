@@ -40,7 +40,7 @@ def _check(got, x, pos, f, a, inter, rot):
 @pytest.mark.parametrize("T,hq,hkv,d,rot", [
     (1, 1, 1, 8, 2), (1, 32, 8, 128, 128), (5, 3, 1, 96, 64), (257, 16, 8, 128, 32),
     (33, 7, 2, 80, 20), (9, 5, 5, 50, 50), (1000, 4, 1, 256, 256), (7, 2, 1, 1024, 1024),
-    (4001, 9, 3, 72, 24)])
+    (4001, 9, 3, 72, 24), (9000, 1, 1, 1024, 1024), (20000, 2, 1, 16, 6)])
 def test_rope(T, hq, hkv, d, rot, inter, dtype):
     g = torch.Generator().manual_seed(T * 7 + d)
     q = torch.randn(T, hq, d, generator=g).to(dtype).cuda()

@@ -146,6 +146,10 @@ def _append(**kw):
     (dict(sc=P(10 * BIG + 4)), ERR_ALIGNMENT), (dict(q=P(BIG + 2)), ERR_ALIGNMENT),
     (dict(qo=P(BIG)), ERR_INVALID_ARG),        # dense rows over the fused buffer
     (dict(qo=P(BIG + 512)), ERR_INVALID_ARG),  # over k
+    (dict(vc=P(8 * BIG)), ERR_INVALID_ARG),    # one pool for both
+    (dict(vc=P(8 * BIG + 4 * 256 * 256 - 16)), ERR_INVALID_ARG),
+    (dict(k=P(8 * BIG + 4096), ks=256), ERR_INVALID_ARG),  # rows of the pool itself
+    (dict(qo=P(9 * BIG + 512)), ERR_INVALID_ARG),
 ])
 def test_rope_append_refused(kw, code):
     assert _append(**kw) == code
@@ -193,6 +197,9 @@ def test_attention_fp8b_refused():
     assert call(sc=P(3 * BIG + 8)) == ERR_ALIGNMENT
     assert call(nb=1 << 24, page=256) == ERR_UNSUPPORTED  # 2^32 cache rows
     assert call(rows=-1) == ERR_INVALID_ARG
+    assert call(mk=(1 << 30) + 1, bts=1 << 23) == ERR_UNSUPPORTED
+    assert call(out=P(BIG + 16)) == ERR_INVALID_ARG  # shifted onto q
+    assert call(mq=17, rows=0) == ERR_INVALID_ARG    # prompts without their key count
     assert call(B=0) == OK
     assert call(T=0) == OK
     assert call(mq=0) == OK
