@@ -210,6 +210,14 @@ extern "C" int nvkv_load_kvcache_fp8b(const void* k_cache, const void* v_cache,
       ((uintptr_t)kv_scale & 7u) || ((uintptr_t)slots & 7u))
     return set_error(NVKV_ERR_ALIGNMENT,
                      "load_kvcache_fp8b: caches and outputs 16-byte, scales and slots 8-byte aligned");
+  const uint64_t out_bytes = (uint64_t)num_slots * num_kv_heads * kBD * 2;
+  const uint64_t pool = (uint64_t)num_blocks * page_size * num_kv_heads * kBD;
+  bool meet = spans_meet(k_out, out_bytes, v_out, out_bytes);
+  for (const void* o : {k_out, v_out})
+    meet |= spans_meet(o, out_bytes, k_cache, pool) || spans_meet(o, out_bytes, v_cache, pool) ||
+            spans_meet(o, out_bytes, kv_scale, pool / (kBBlock * kBD) * 8);
+  if (meet)
+    return set_error(NVKV_ERR_INVALID_ARG, "load_kvcache_fp8b: an output overlaps another or the pool");
   const int lanes = num_kv_heads == 1 ? 16 : 32;  // 16 chunks of 8 codes a head
   const int64_t rows = 256 / lanes;                // a CTA's
   const unsigned blocks = (unsigned)std::min<int64_t>((num_slots + rows - 1) / rows, 148 * 16);

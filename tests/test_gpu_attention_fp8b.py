@@ -319,3 +319,24 @@ def test_two_streams_at_once_and_in_place():
         assert torch.equal(out, want)
         nvkv.paged_attention_fp8b(q, *pool, cq, ck, bt, 1, mk, D ** -0.5, out=q, workspace=ws)
         assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_mixed_batch_in_place_with_padding(dtype):
+    """Prompts, chunks, single rows and padded entries, out = q: the bits of a call
+    into another buffer, and rows behind the last sequence as they were."""
+    q_lens = [150, 1, 0, 300, 1, 17, 0]
+    k_lens = [150, 2000, 5, 1100, 1, 17, 1]
+    pool, bt, rows = filled(k_lens, 2, seed=41, dtype=dtype)
+    q = _q(sum(q_lens) + 5, 8, dtype, 41)
+    out = torch.full_like(q, 7.0)
+    kw = dict(prompt_kv_tokens=150 + 1100 + 17)
+    args = (*pool, cu(q_lens), cu(k_lens), bt, 300, 2000, D ** -0.5)
+    nvkv.paged_attention_fp8b(q, *args, out=out, **kw)
+    torch.cuda.synchronize()
+    assert nvkv.device_error() == 0 and bool((out[-5:] == 7).all())
+    check_attention(out, q, rows, q_lens, k_lens, D ** -0.5, prompt_err(dtype))
+    before = q.clone()
+    nvkv.paged_attention_fp8b(q, *args, out=q, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(q[:-5], out[:-5]) and torch.equal(q[-5:], before[-5:])

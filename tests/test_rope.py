@@ -171,6 +171,9 @@ def test_load_refused():
     assert call(hkv=0) == ERR_INVALID_ARG
     assert call(ko=None) == ERR_INVALID_ARG
     assert call(ko=P(4 * BIG + 8)) == ERR_ALIGNMENT
+    assert call(vo=P(4 * BIG + 1024)) == ERR_INVALID_ARG  # onto k_out
+    assert call(ko=P(BIG + 1024)) == ERR_INVALID_ARG      # into the pool
+    assert call(vo=P(2 * BIG)) == ERR_INVALID_ARG         # onto the scales
     assert call(n=0, kc=None, sc=None, slots=None, ko=None, vo=None) == OK
 
 
