@@ -585,17 +585,16 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     alive = alive && __all_sync(0xffffffffu,
                                 mbar_wait(&q_full[qb], (part >> 1) & 1, p.err));
     bar_compute();  // rowlim
-    // a row's factor and last visible key, in registers where there is room
-    constexpr bool kRegs = HP <= 8;
+    constexpr bool kRegs = HP <= 16;  // the rows' factors, in registers where there is room
     float rf_r[kRegs ? HP : 1];
-    int lim_r[kRegs ? HP : 1];
     if constexpr (kRegs) {
 #pragma unroll
-      for (int r = 0; r < HP; ++r) rf_r[r] = rowf[qb * HP + r], lim_r[r] = rowlim[r];
+      for (int r = 0; r < HP; ++r) rf_r[r] = rowf[qb * HP + r];
     }
-    float M[HP], l[HP];
+    float M[HP], l[HP];  // (unused rows: no score passes infinity, every weight is 0)
 #pragma unroll
-    for (int r = 0; r < HP; ++r) M[r] = -INFINITY, l[r] = 0.f;
+    for (int r = 0; r < HP; ++r) M[r] = r < rows ? -INFINITY : INFINITY, l[r] = 0.f;
+    const int seen = p.causal ? k_len - sq_info.q_len + 1 : k_len;  // keys that every row sees
     for (int i = 0; i < n_tiles; ++i, ++it) {
       const int s = st, x = it & 1;
       alive = alive && mbar_ready(&s_full[x], (it >> 1) & 1, p.err) &&
@@ -636,10 +635,14 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
 #pragma unroll
       for (int r = 0; r < HP; ++r) {
         const float f = kRegs ? rf_r[kRegs ? r : 0] : rowf[qb * HP + r];
-        z[r] = j <= (kRegs ? lim_r[kRegs ? r : 0] : rowlim[r]) ? z[r] * (f * ks) + (float)ev
-                                                               : -INFINITY;
-        over |= z[r] > M[r] + kHeadroom;
+        z[r] = z[r] * (f * ks) + (float)ev;
       }
+      if ((cur.t + i + 1) * kBTile > seen) {
+#pragma unroll
+        for (int r = 0; r < HP; ++r) z[r] = j <= rowlim[r] ? z[r] : -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < HP; ++r) over |= z[r] > M[r] + kHeadroom;
       if (bar_compute_any(over)) {
         // new maxima: of the warp's keys, lane r keeping row r's, then of the four warps'
         float mine = -INFINITY;
@@ -731,19 +734,39 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[(it - 1) & 1],
                                                        ((it - 1) >> 1) & 1, p.err));
     tc_fence_after();
+    // row sums: of the warp, each step of the first ones halving the rows a lane
+    // keeps, then of the four warps; lane r goes on with row r
+    int m = 16;
 #pragma unroll
-    for (int r = 0; r < HP; ++r) {
-      float v = l[r];
+    for (int half = HP / 2; half >= 1; half >>= 1, m >>= 1) {
+      const bool up = lane & m;
 #pragma unroll
-      for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-      if (lane == 0) red[warp * HP + r] = v;
+      for (int r = 0; r < half; ++r) {
+        const float send = up ? l[r] : l[r + half], keep = up ? l[r + half] : l[r];
+        l[r] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+      }
     }
-    bar_compute();
+    for (; m >= 1; m >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], m);
+    if (lane % (32 / HP) == 0) red[warp * HP + lane / (32 / HP)] = l[0];
+    bar_compute();  // (the next part's first one is before the next write to red)
     const bool whole = n_tiles == sq_info.tiles;
     const int slot = 2 * cta + (cur.t == 0 ? 1 : 0);
     if (!whole && key == 0)
       p.ws_desc[slot] = make_int2(alive ? cur.b : -1, cur.t + n_tiles == sq_info.tiles);
+    const int r_ = lane % HP;
+    const float ls = red[r_] + red[HP + r_] + red[2 * HP + r_] + red[3 * HP + r_];
+    const float inv = ls == 0.f ? 0.f : 1.f / (ls * kWeight);
+    int64_t at = (int64_t)slot * (p.q_cap * p.group) + r_;
+    if (whole) {
+      at = (int64_t)(q0 + r_ / p.group) * p.hq + kvh * p.group + r_ % p.group;
+    } else if (warp == 0 && lane < rows && alive) {
+      float Mr = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < HP; ++r) Mr = r == lane ? M[r] : Mr;
+      p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr + log2f(ls);
+    }
     constexpr int n = HP == 4 ? 4 : 8;
+#pragma unroll
     for (int c = 0; c < HP; c += n) {
       float o[kPPieces][n];
 #pragma unroll
@@ -751,26 +774,15 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        const int r = c + i;
-        if (r >= rows || !alive) continue;
-        const float ls = red[r] + red[HP + r] + red[2 * HP + r] + red[3 * HP + r];
-        const float acc = (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2 +
-                           o[3][i] * kPiece3) * (1.f / kWeight);
-        const float val = ls == 0.f ? 0.f : acc / ls;
-        if (whole) {
-          const int64_t at = (int64_t)(q0 + r / p.group) * p.hq + kvh * p.group + r % p.group;
-          static_cast<T*>(p.out)[at * kBD + key] = DT<T>::from_f(val);
-        } else {
-          const int64_t at = (int64_t)slot * (p.q_cap * p.group) + r;
-          p.ws_o[at * kBD + key] = val;
-          float Mr = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < HP; ++k) Mr = k == r ? M[k] : Mr;
-          if (key == 0) p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr + log2f(ls);
-        }
+        const float w = __shfl_sync(0xffffffffu, inv, c + i);
+        const float val = w == 0.f ? 0.f : (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2 +
+                                            o[3][i] * kPiece3) * w;
+        const int64_t to = __shfl_sync(0xffffffffu, at, c + i) * kBD + key;
+        if (c + i >= rows || !alive) continue;
+        if (whole) static_cast<T*>(p.out)[to] = DT<T>::from_f(val);
+        else p.ws_o[to] = val;
       }
     }
-    bar_compute();  // the sums have been read
     }
   }
 
