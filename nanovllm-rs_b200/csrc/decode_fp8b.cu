@@ -765,22 +765,33 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       for (int r = 0; r < HP; ++r) Mr = r == lane ? M[r] : Mr;
       p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr + log2f(ls);
     }
-    constexpr int n = HP == 4 ? 4 : 8;
+    // four rows a step, their chains side by side; not unrolled, as this runs once a
+    // part and mostly from a cold instruction cache
+#pragma unroll 1
+    for (int c = 0; c < rows; c += 4) {
+      float o[kPPieces][4], val[4];
+      int64_t to[4];
 #pragma unroll
-    for (int c = 0; c < HP; c += n) {
-      float o[kPPieces][n];
+      for (int pc = 0; pc < kPPieces; ++pc) tmem_ldn<4>(lane_addr + 2 * kCols + pc * HP + c, o[pc]);
 #pragma unroll
-      for (int pc = 0; pc < kPPieces; ++pc) tmem_ldn<n>(lane_addr + 2 * kCols + pc * HP + c, o[pc]);
+      for (int i = 0; i < 4; ++i) {
+        val[i] = __shfl_sync(0xffffffffu, inv, c + i);
+        to[i] = __shfl_sync(0xffffffffu, at, c + i) * kBD + key;
+      }
       tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const float w = __shfl_sync(0xffffffffu, inv, c + i);
-        const float val = w == 0.f ? 0.f : (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2 +
-                                            o[3][i] * kPiece3) * w;
-        const int64_t to = __shfl_sync(0xffffffffu, at, c + i) * kBD + key;
-        if (c + i >= rows || !alive) continue;
-        if (whole) static_cast<T*>(p.out)[to] = DT<T>::from_f(val);
-        else p.ws_o[to] = val;
+      for (int i = 0; i < 4; ++i)
+        val[i] = val[i] == 0.f ? 0.f : (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2 +
+                                        o[3][i] * kPiece3) * val[i];
+      const int n = alive ? rows - c : 0;
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) static_cast<T*>(p.out)[to[i]] = DT<T>::from_f(val[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) p.ws_o[to[i]] = val[i];
       }
     }
     }
