@@ -53,7 +53,6 @@ constexpr int kBTile = 128;                   // keys a tile
 constexpr int kBCode = kBTile * kBD;          // 16 KB of codes
 constexpr int kBStage = 2 * kBCode;           // K, V
 constexpr int kBScale = kBTile / NVKV_FP8B_BLOCK * 2;  // floats of a tile's scales
-constexpr int kBThreads = 256;
 constexpr float kLog2e_ = 1.4426950408889634f;
 // Q and the weights P as sums of e4m3 pieces, x = c0 + 2^-5 c1 + 2^-10 c2 + ...,
 // every piece the e4m3 rounding of what the ones before left over (at most 8 of a
@@ -75,6 +74,9 @@ template <int HP>
 struct Cfg {
   static constexpr int kCols = (kQPieces * HP + 15) / 16 * 16;  // pieces as B columns
   static constexpr int kPCols = kPPieces * HP;
+  // compute warpgroups, each with its rows of a tile
+  static constexpr int kGroups = HP <= 8 ? 1 : HP / 8, kRows = HP / kGroups;
+  static constexpr int kThreads = 128 * kGroups + 128;
   static constexpr int kCtasPerSm = HP <= 8 ? 2 : 1;
   static constexpr int kStages = HP <= 8 ? 3 : HP == 16 ? 6 : 5;
   static constexpr int kQBytes = kCols * 128;
@@ -226,17 +228,20 @@ __device__ __forceinline__ bool mbar_ready(uint64_t* bar, uint32_t parity, int* 
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-// The compute warps' barrier, returning whether any thread's flag was set.
-__device__ __forceinline__ bool bar_compute_any(bool flag) {
+// The barrier of a compute warpgroup
+__device__ __forceinline__ void bar_compute(int g) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
+}
+// and returning whether any thread's flag was set.
+__device__ __forceinline__ bool bar_compute_any(int g, bool flag) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)flag)
+      : "r"((uint32_t)flag), "r"(1 + g)
       : "memory");
   return r != 0;
 }
@@ -330,11 +335,12 @@ __device__ __forceinline__ void load_q(const Params& p, uint32_t q0, int kvh, in
 }
 
 template <typename T, int HP>
-__global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
+__global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
     decode_fp8b_kernel(const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const Params p) {
   using C = Cfg<HP>;
-  constexpr int kStages = C::kStages, kCols = C::kCols;
+  constexpr int kStages = C::kStages, kCols = C::kCols, kThreads = C::kThreads, R = C::kRows;
+  constexpr int kTma = 4 * C::kGroups, kMma = kTma + 1, kLoadQ = kTma + 2;  // warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -353,12 +359,12 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
   uint64_t* q_empty = q_full + 2;      // [2] its last scores are done, its factors read
   uint64_t* drain = q_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  __shared__ int64_t sums[9];
+  __shared__ int64_t sums[kThreads / 32];
   __shared__ int start_b, start_t;
 
   const int cta = blockIdx.x, share = cta / p.hkv, kvh = cta % p.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 128) {
+  if (threadIdx.x == kTma * 32) {
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
@@ -371,20 +377,20 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 128);
+      mbar_init(&p_full[x], 128 * C::kGroups);
       mbar_init(&o_done[x], 1);
       mbar_init(&q_full[x], 64);
-      mbar_init(&q_empty[x], 129);
+      mbar_init(&q_empty[x], 128 * C::kGroups + 1);
     }
     mbar_init(drain, 1);
     fence_mbar_init();
   }
-  for (int i = threadIdx.x; i < (C::kQStride + C::kQBytes) / 16; i += kBThreads)  // the unused columns
+  for (int i = threadIdx.x; i < (C::kQStride + C::kQBytes) / 16; i += kThreads)  // the unused columns
     *reinterpret_cast<uint4*>(sq + i * 16) = make_uint4(0, 0, 0, 0);
   pdl_wait();  // inputs may come from the kernel before this one
 
   // ---- this CTA's share of the tiles: [lo, hi) of their total ----
-  const int each = (p.num_seqs + kBThreads - 1) / kBThreads;  // sequences a thread
+  const int each = (p.num_seqs + kThreads - 1) / kThreads;  // sequences a thread
   const int b_lo = threadIdx.x * each, b_hi = min(b_lo + each, p.num_seqs);
   int64_t mine = 0;
   for (int b = b_lo; b < b_hi; ++b) {
@@ -409,7 +415,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
-  for (int w = 0; w < kBThreads / 32; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) upto += sums[w];
     total += sums[w];
   }
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       at += n;
     }
   }
-  if (warp == 5) {
+  if (warp == kMma) {
     tmem_alloc(tmem_slot, C::kTmem);
     tmem_relinquish();
   }
@@ -445,7 +451,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
   Seq sq_info;
   int n_tiles;
 
-  if (warp == 4) {
+  if (warp == kTma) {
     // ------------------------------ TMA producer ------------------------------
     int it = 0, go = 1;
     while (go && cur.next(p, sq_info, n_tiles, lane)) {
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     if (!go && lane == 0)  // given up: wait for the copies in flight
       for (int i = max(0, it - kStages); i < it; ++i)
         mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err);
-  } else if (warp == 5) {
+  } else if (warp == kMma) {
     // ------------------------------- MMA issuer -------------------------------
     // The whole warp walks the loop, one lane issues: the loop is the critical path
     // of a tile, so descriptors move by 32-bit adds and ring positions by compares.
@@ -547,7 +553,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       tc_commit(drain);
       mbar_wait(drain, 0, nullptr);
     }
-  } else if (warp >= 6) {
+  } else if (warp >= kLoadQ) {
     // -------------------------------- Q loaders --------------------------------
     int part = 0;
     bool ok = true;
@@ -558,7 +564,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
                                                      p.err));
       if (ok) {
         load_q<T, HP>(p, sq_info.q0, kvh, sq_info.q_len * p.group, sq + qb * C::kQStride,
-                      rowf + qb * HP, warp - 6, lane);
+                      rowf + qb * HP, warp - kLoadQ, lane);
         fence_async_smem();
         mbar_arrive(&q_full[qb]);
       }
@@ -567,8 +573,9 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     }
   } else {
     // ------------------------------ compute warps ------------------------------
-    const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
-    const int key = threadIdx.x;  // this thread's key of a tile, and its dim of O
+    const int grp = C::kGroups == 1 ? 0 : warp / 4, wg = warp % 4, r0 = grp * R;  // rows r0 ..
+    const uint32_t lane_addr = tmem + ((uint32_t)(wg * 32) << 16);
+    const int key = threadIdx.x % 128;  // this thread's key of a tile, and its dim of O
     bool alive = true;
     int it = 0, part = 0, st = 0;  // st, st_ph: ring position
     uint32_t st_ph = 0;
@@ -576,24 +583,22 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     const int qb = part & 1;
     const int rows = sq_info.q_len * p.group, k_len = sq_info.k_len;
     const uint32_t q0 = sq_info.q0;
-    if (threadIdx.x < HP) {
-      const int r = threadIdx.x;
+    if (key < R) {
+      const int r = r0 + key;
       rowlim[r] = r >= rows ? -1 : p.causal ? k_len - sq_info.q_len + r / p.group : k_len - 1;
     }
     // a wait that runs out is not repeated, but the warp stays in step with the
     // others' barriers to the end of the share
     alive = alive && __all_sync(0xffffffffu,
                                 mbar_wait(&q_full[qb], (part >> 1) & 1, p.err));
-    bar_compute();  // rowlim
-    constexpr bool kRegs = HP <= 16;  // the rows' factors, in registers where there is room
-    float rf_r[kRegs ? HP : 1];
-    if constexpr (kRegs) {
+    bar_compute(grp);  // rowlim
+    float M[R], l[R], rf_r[R];  // (unused rows: no score passes infinity, every weight is 0)
 #pragma unroll
-      for (int r = 0; r < HP; ++r) rf_r[r] = rowf[qb * HP + r];
+    for (int r = 0; r < R; ++r) {
+      M[r] = r0 + r < rows ? -INFINITY : INFINITY;
+      l[r] = 0.f;
+      rf_r[r] = rowf[qb * HP + r0 + r];
     }
-    float M[HP], l[HP];  // (unused rows: no score passes infinity, every weight is 0)
-#pragma unroll
-    for (int r = 0; r < HP; ++r) M[r] = r < rows ? -INFINITY : INFINITY, l[r] = 0.f;
     const int seen = p.causal ? k_len - sq_info.q_len + 1 : k_len;  // keys that every row sees
     for (int i = 0; i < n_tiles; ++i, ++it) {
       const int s = st, x = it & 1;
@@ -609,9 +614,9 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       // the upper bound keeps a stale block's NaN out of the masked sums)
       const int ev = min(max((int)(__float_as_uint(sc.y) >> 23 & 0xffu) - 127, -100), 120);
       const int j = (cur.t + i) * kBTile + key;
-      float z[HP];
-      const uint32_t cs = lane_addr + x * kCols;
-      if constexpr (HP == 4) {
+      float z[R];
+      const uint32_t cs = lane_addr + x * kCols + r0;
+      if constexpr (R == 4) {
         float a[16];
         tmem_ld16(cs, a);
         tmem_wait_ld();
@@ -619,66 +624,58 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
         for (int r = 0; r < 4; ++r)
           z[r] = a[r] + a[4 + r] * kPiece1 + a[8 + r] * kPiece2;
       } else {
+        float a0[8], a1[8], a2[8];
+        tmem_ldn<8>(cs, a0);
+        tmem_ldn<8>(cs + HP, a1);
+        tmem_ldn<8>(cs + 2 * HP, a2);
+        tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < HP; c += 8) {
-          float a0[8], a1[8], a2[8];
-          tmem_ldn<8>(cs + c, a0);
-          tmem_ldn<8>(cs + HP + c, a1);
-          tmem_ldn<8>(cs + 2 * HP + c, a2);
-          tmem_wait_ld();
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            z[c + r] = a0[r] + a1[r] * kPiece1 + a2[r] * kPiece2;
-        }
+        for (int r = 0; r < 8; ++r)
+          z[r] = a0[r] + a1[r] * kPiece1 + a2[r] * kPiece2;
       }
       bool over = false;  // a score past its row's headroom
 #pragma unroll
-      for (int r = 0; r < HP; ++r) {
-        const float f = kRegs ? rf_r[kRegs ? r : 0] : rowf[qb * HP + r];
-        z[r] = z[r] * (f * ks) + (float)ev;
-      }
+      for (int r = 0; r < R; ++r) z[r] = z[r] * (rf_r[r] * ks) + (float)ev;
       if ((cur.t + i + 1) * kBTile > seen) {
 #pragma unroll
-        for (int r = 0; r < HP; ++r) z[r] = j <= rowlim[r] ? z[r] : -INFINITY;
+        for (int r = 0; r < R; ++r) z[r] = j <= rowlim[r0 + r] ? z[r] : -INFINITY;
       }
 #pragma unroll
-      for (int r = 0; r < HP; ++r) over |= z[r] > M[r] + kHeadroom;
-      if (bar_compute_any(over)) {
+      for (int r = 0; r < R; ++r) over |= z[r] > M[r] + kHeadroom;
+      if (bar_compute_any(grp, over)) {
         // new maxima: of the warp's keys, lane r keeping row r's, then of the four warps'
         float mine = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < HP; ++r) {
+        for (int r = 0; r < R; ++r) {
           const float m = redux_max(z[r]);
           if (lane == r) mine = m;
         }
-        if (lane < HP) red[warp * HP + lane] = mine;
-        bar_compute();
-        float fac[HP];
+        if (lane < R) red[wg * HP + r0 + lane] = mine;
+        bar_compute(grp);
+        float fac[R];
 #pragma unroll
-        for (int r = 0; r < HP; ++r) {
-          const float m = fmaxf(fmaxf(red[r], red[HP + r]), fmaxf(red[2 * HP + r], red[3 * HP + r]));
+        for (int r = 0; r < R; ++r) {
+          const float* x = red + r0 + r;
+          const float m = fmaxf(fmaxf(x[0], x[HP]), fmaxf(x[2 * HP], x[3 * HP]));
           const bool up = m > M[r] + kHeadroom;
           fac[r] = up ? ex2_mufu(M[r] - m) : 1.f;
           M[r] = up ? m : M[r];
           l[r] *= fac[r];
         }
-        bar_compute();  // (the next exchange may be the next tile's)
+        bar_compute(grp);  // (the next exchange may be the next tile's)
         if (i > 0) {  // O is in units of 2^M
           alive = alive && mbar_ready(&o_done[x ^ 1], ((it - 1) >> 1) & 1, p.err);
           tc_fence_after();
-          constexpr int n = HP == 4 ? 4 : 8;
 #pragma unroll
-          for (int pc = 0; pc < kPPieces; ++pc)
-#pragma unroll
-            for (int c = 0; c < HP; c += n) {
-              const uint32_t a = lane_addr + 2 * kCols + pc * HP + c;
-              float o[n];
-              tmem_ldn<n>(a, o);
+          for (int pc = 0; pc < kPPieces; ++pc) {
+              const uint32_t a = lane_addr + 2 * kCols + pc * HP + r0;
+              float o[R];
+              tmem_ldn<R>(a, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int r = 0; r < n; ++r) o[r] *= fac[c + r];
+              for (int r = 0; r < R; ++r) o[r] *= fac[r];
               const uint32_t* w = reinterpret_cast<const uint32_t*>(o);
-              if constexpr (n == 4)
+              if constexpr (R == 4)
                 asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a),
                              "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                              : "memory");
@@ -695,9 +692,9 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       }
       // weights, scaled for the pieces; the row sums without the V scale
       const float unscale = __uint_as_float((uint32_t)(127 - ev) << 23);
-      uint32_t w[C::kPCols / 4];
+      uint32_t w[kPPieces * R / 4];
 #pragma unroll
-      for (int c = 0; c < HP; c += 4) {
+      for (int c = 0; c < R; c += 4) {
         float e[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -709,16 +706,24 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
         uint32_t pw[kPPieces];
         pieces4(e[0], e[1], e[2], e[3], pw);
 #pragma unroll
-        for (int pc = 0; pc < kPPieces; ++pc) w[(pc * HP + c) / 4] = pw[pc];
+        for (int pc = 0; pc < kPPieces; ++pc) w[(pc * R + c) / 4] = pw[pc];
       }
       if (it >= 2)  // this buffer's last reader
         alive = alive && mbar_ready(&o_done[x], ((it - 2) >> 1) & 1, p.err);
       uint8_t* dst = sp + x * C::kPBytes + key * 16;
+      if constexpr (C::kGroups == 1) {
 #pragma unroll
-      for (int nb = 0; nb < C::kPCols / 16; ++nb)
-        *reinterpret_cast<uint4*>(dst + nb * 2048) =
-            make_uint4(w[4 * nb], w[4 * nb + 1], w[4 * nb + 2], w[4 * nb + 3]);
-      if (j >= k_len) {  // a key past the end: its V row may hold NaN codes, and 0 x NaN is NaN
+        for (int nb = 0; nb < C::kPCols / 16; ++nb)
+          *reinterpret_cast<uint4*>(dst + nb * 2048) =
+              make_uint4(w[4 * nb], w[4 * nb + 1], w[4 * nb + 2], w[4 * nb + 3]);
+      } else {  // piece pc of these eight rows is half of a block of 16 columns
+#pragma unroll
+        for (int pc = 0; pc < kPPieces; ++pc) {
+          const int n = pc * HP + r0;
+          *reinterpret_cast<uint2*>(dst + n / 16 * 2048 + n % 16) = make_uint2(w[2 * pc], w[2 * pc + 1]);
+        }
+      }
+      if (grp == 0 && j >= k_len) {  // a key past the end: its V row may hold NaN codes, and 0 x NaN is NaN
         uint8_t* vr = smem + s * kBStage + kBCode + key * 128;
 #pragma unroll
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vr + c * 16) = make_uint4(0, 0, 0, 0);
@@ -738,7 +743,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
     // keeps, then of the four warps; lane r goes on with row r
     int m = 16;
 #pragma unroll
-    for (int half = HP / 2; half >= 1; half >>= 1, m >>= 1) {
+    for (int half = R / 2; half >= 1; half >>= 1, m >>= 1) {
       const bool up = lane & m;
 #pragma unroll
       for (int r = 0; r < half; ++r) {
@@ -747,32 +752,32 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       }
     }
     for (; m >= 1; m >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], m);
-    if (lane % (32 / HP) == 0) red[warp * HP + lane / (32 / HP)] = l[0];
-    bar_compute();  // (the next part's first one is before the next write to red)
+    if (lane % (32 / R) == 0) red[wg * HP + r0 + lane / (32 / R)] = l[0];
+    bar_compute(grp);  // (the next part's first one is before the next write to red)
     const bool whole = n_tiles == sq_info.tiles;
     const int slot = 2 * cta + (cur.t == 0 ? 1 : 0);
-    if (!whole && key == 0)
+    if (!whole && threadIdx.x == 0)
       p.ws_desc[slot] = make_int2(alive ? cur.b : -1, cur.t + n_tiles == sq_info.tiles);
-    const int r_ = lane % HP;
+    const int r_ = r0 + lane % R;
     const float ls = red[r_] + red[HP + r_] + red[2 * HP + r_] + red[3 * HP + r_];
     const float inv = ls == 0.f ? 0.f : 1.f / (ls * kWeight);
     int64_t at = (int64_t)slot * (p.q_cap * p.group) + r_;
     if (whole) {
       at = (int64_t)(q0 + r_ / p.group) * p.hq + kvh * p.group + r_ % p.group;
-    } else if (warp == 0 && lane < rows && alive) {
+    } else if (wg == 0 && lane < R && r_ < rows && alive) {
       float Mr = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < HP; ++r) Mr = r == lane ? M[r] : Mr;
+      for (int r = 0; r < R; ++r) Mr = r == lane ? M[r] : Mr;
       p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr + log2f(ls);
     }
     // four rows a step, their chains side by side; not unrolled, as this runs once a
     // part and mostly from a cold instruction cache
 #pragma unroll 1
-    for (int c = 0; c < rows; c += 4) {
+    for (int c = 0; c < R && r0 + c < rows; c += 4) {
       float o[kPPieces][4], val[4];
       int64_t to[4];
 #pragma unroll
-      for (int pc = 0; pc < kPPieces; ++pc) tmem_ldn<4>(lane_addr + 2 * kCols + pc * HP + c, o[pc]);
+      for (int pc = 0; pc < kPPieces; ++pc) tmem_ldn<4>(lane_addr + 2 * kCols + pc * HP + r0 + c, o[pc]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         val[i] = __shfl_sync(0xffffffffu, inv, c + i);
@@ -783,7 +788,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
       for (int i = 0; i < 4; ++i)
         val[i] = val[i] == 0.f ? 0.f : (o[0][i] + o[1][i] * kPiece1 + o[2][i] * kPiece2 +
                                         o[3][i] * kPiece3) * val[i];
-      const int n = alive ? rows - c : 0;
+      const int n = alive ? rows - r0 - c : 0;
       if (whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -800,7 +805,7 @@ __global__ void __launch_bounds__(kBThreads, Cfg<HP>::kCtasPerSm)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) {
+  if (warp == kMma) {
     __syncwarp();
     tmem_dealloc(tmem, C::kTmem);
   }
@@ -876,7 +881,7 @@ int launch(const AttnArgs& a, const Params& p, const CUtensorMap& mk, const CUte
   static unsigned long long done = 0;
   int rc = ensure_smem_attr((const void*)kern, Cfg<HP>::kSmem, &done);
   if (!rc)
-    rc = launch_pdl(kern, dim3(p.groups * a.hkv), dim3(kBThreads), Cfg<HP>::kSmem, a.stream,
+    rc = launch_pdl(kern, dim3(p.groups * a.hkv), dim3(Cfg<HP>::kThreads), Cfg<HP>::kSmem, a.stream,
                     "decode fp8b launch", mk, mv, p);
   if (!rc)
     rc = launch_pdl(combine_fp8b_kernel<T>, dim3(p.groups * a.hkv, p.q_cap * p.group), dim3(kBD), 0,
