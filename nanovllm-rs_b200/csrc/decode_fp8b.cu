@@ -225,6 +225,14 @@ __device__ __forceinline__ bool mbar_ready(uint64_t* bar, uint32_t parity, int* 
   if (__all_sync(0xffffffffu, ok)) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
+// One lane of the (converged) warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -512,7 +520,7 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
       ok = ok && mbar_ready(&p_full[x], ((uint32_t)(it - 1) >> 1) & 1u, p.err);
       if (!ok) return;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t v = v0 + o_st * (kBStage >> 4), pb = p0 + x * (C::kPBytes >> 4);
 #pragma unroll
         for (uint32_t kk = 0; kk < 4; ++kk)
@@ -532,7 +540,7 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
         ok = ok && mbar_ready(&full[s_st], s_ph, p.err);
         if (ok) {  // S(it): K-major codes, 32 dims a step
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             const uint32_t k = k0 + s_st * (kBStage >> 4);
 #pragma unroll
             for (uint32_t kk = 0; kk < 4; ++kk)
@@ -549,7 +557,7 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
       }
     }
     issue_o();
-    if (lane == 0 && !ok) {  // given up: let the products in flight finish before the memory goes
+    if (!ok && elect_one()) {  // given up: let the products in flight finish before the memory goes
       tc_commit(drain);
       mbar_wait(drain, 0, nullptr);
     }
