@@ -14,7 +14,8 @@ Cases (one JSON line each; bytes/flops are the algorithmic figures):
   decode_32b_tp8  Qwen3-32B TP8 per GPU: B=64, 8q/1kv, L=32768            (HBM)
   decode_*_fp8b   the same decode layers over the block-scaled pool
                   (nvkv_paged_attention_fp8b)                            (HBM)
-  verify_8b_tp1_fp8b  64 sequences x 4 new tokens over that pool         (HBM)
+  verify_*_fp8b   64 sequences x 4 new tokens over that pool, 16 and 32
+                  query rows a kv head                                   (HBM)
   rope_prefill    nvkv_rope, 16384 tokens, 32q/8kv heads                 (HBM)
   append_fp8b_*   nvkv_rope_append into the block-scaled pool, a 256-token
                   decode step and 16 prompts x 1024                      (HBM)
@@ -559,6 +560,10 @@ CASES = {
         8),
     "decode_32b_tp8_fp8b": lambda it: case_decode_fp8b(
         "decode_32b_tp8_fp8b", np.full(64, 32768), 8, 1, 64 * 128 + 2, it, 2),
+    "decode_g16_fp8b": lambda it: case_decode_fp8b(
+        "decode_g16_fp8b", np.random.default_rng(8).integers(2048, 4097, 64), 16, 1, 1100, it, 8),
+    "verify_g8_fp8b": lambda it: case_decode_fp8b(
+        "verify_g8_fp8b", np.full(64, 2000), 32, 4, 64 * 8, it, 4, new=4),
     "verify_8b_tp1_fp8b": lambda it: case_decode_fp8b(
         "verify_8b_tp1_fp8b", np.full(64, 2000), 32, 8, 64 * 8, it, 2, new=4),
     "rope_prefill": lambda it: case_rope(16384, it),

@@ -11,23 +11,24 @@
 // (the tensor core's N has room), and are joined in f32 with their weights where
 // the columns are read.
 //
-// A compute thread owns one key of the tile (one TMEM lane): it joins its
-// scores, multiplies by the key block's K scale, and forms z = S + log2(V
-// scale), so a weight 2^(z - M) already carries the value's scale and O needs
-// none; the row sum takes the scale back out (an exact power of two).  M is a
+// A compute thread owns one key of the tile (one TMEM lane) and up to 8 of its
+// rows: it joins its scores, multiplies by the key block's K scale, and forms z =
+// S + log2(V scale), so a weight 2^(z - M) already carries the value's scale and O
+// needs none; the row sum takes the scale back out (an exact power of two).  M is a
 // row's maximum of z over the CTA's keys, to within a headroom: one barrier with a
 // reduced flag a tile says whether any score has left it; only then are maxima
 // joined (redux.sync in a warp, shared memory over the four) and O rescaled in
-// TMEM.  Weights leave as one or
-// more 16-byte stores a thread (N-major B operand).
+// TMEM.  Weights leave as 8- or 16-byte stores (N-major B operand).
 //
-//   warps 0-3  compute (TMEM lanes 32 w .. 32 w + 31)
-//   warp 4     TMA producer: K and V code tiles (SWIZZLE_128B) and the tile's
+//   G warpgroups  compute, G = 1, or rows / 8 for 16 and 32 rows (a warp has TMEM
+//              lanes 32 (w % 4) ..): the chain of a tile, not its issue, sets their
+//              pace, so rows go side by side
+//   a warp     TMA producer: K and V code tiles (SWIZZLE_128B) and the tile's
 //              64 bytes of scales, an mbarrier ring
-//   warp 5     TMEM allocation and every tcgen05.mma, one thread, in the order
+//   a warp     TMEM allocation and every tcgen05.mma, one thread, in the order
 //              S(0), S(1), O(0), S(2), O(1), ...: a tile's scores are computed
 //              while the tile before it is in the softmax
-//   warps 6-7  the next sequence's Q pieces
+//   two warps  the next sequence's Q pieces
 //
 // Work.  One wave of persistent CTAs, a group of Hkv neighbours (one per kv head)
 // for each share of the batch: the sequences' tiles, one after the other, are cut
@@ -38,8 +39,13 @@
 // through, each CTA leaves f32 partials and a base-2 log-sum-exp in the workspace
 // (at most two per CTA), and combine_fp8b_kernel joins them.
 //
-// Bound by HBM: 2 x 128 bytes of codes + 0.5 of scales a key and kv head; per
-// tile the compute warps issue ~700 instructions for 32 KB.
+// Bound by HBM up to 8 rows: 2 x 128 bytes of codes + 0.5 of scales a key and kv
+// head.  256 sequences of ~1290 keys, 32 / 8 heads (681 MB): 114.8 us, 5.9 TB/s of
+// the 6.55 that a copy reaches; the same loads without products 96 us.  64 x 32768
+// keys, 8 / 1 heads: 90.2 us, 6.0 TB/s.  16 rows (64 x 2000 keys, 32 / 8 heads, 4
+// queries each, 267 MB): 80 us, bound by the tile's chain of scores, weights and the
+// issue of 8 products; one warpgroup for all 16 rows took 87, and 2 CTAs of 2 stages
+// instead of one of 6 then 85 (but 31.5 against 30.6 at 64 x 3000 keys of one head).
 #include <algorithm>
 #include <type_traits>
 
@@ -258,21 +264,20 @@ __device__ __forceinline__ float redux_max(float x) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
-// n (4, 8, 16) consecutive f32 columns of this thread's TMEM lane
+// n (4 or 8) consecutive f32 columns of this thread's TMEM lane
 template <int n>
 __device__ __forceinline__ void tmem_ldn(uint32_t a, float* v) {
+  static_assert(n == 4 || n == 8, "tmem_ldn");
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   if constexpr (n == 4)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(a));
-  else if constexpr (n == 8)
+  else
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
                    "=r"(r[6]), "=r"(r[7])
                  : "r"(a));
-  else
-    tmem_ld16(a, v);
 }
 
 // e4m3 codes of (a, b), low byte a
@@ -676,25 +681,25 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
           tc_fence_after();
 #pragma unroll
           for (int pc = 0; pc < kPPieces; ++pc) {
-              const uint32_t a = lane_addr + 2 * kCols + pc * HP + r0;
-              float o[R];
-              tmem_ldn<R>(a, o);
-              tmem_wait_ld();
+            const uint32_t a = lane_addr + 2 * kCols + pc * HP + r0;
+            float o[R];
+            tmem_ldn<R>(a, o);
+            tmem_wait_ld();
 #pragma unroll
-              for (int r = 0; r < R; ++r) o[r] *= fac[r];
-              const uint32_t* w = reinterpret_cast<const uint32_t*>(o);
-              if constexpr (R == 4)
-                asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a),
-                             "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                             : "memory");
-              else
-                asm volatile(
-                    "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(
-                        a),
-                    "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
-                    "r"(w[7])
-                    : "memory");
-            }
+            for (int r = 0; r < R; ++r) o[r] *= fac[r];
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(o);
+            if constexpr (R == 4)
+              asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a),
+                           "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                           : "memory");
+            else
+              asm volatile(
+                  "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(
+                      a),
+                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                  "r"(w[7])
+                  : "memory");
+          }
           tmem_wait_st();
         }
       }

@@ -51,8 +51,8 @@ __device__ __forceinline__ void store_values(T* dst, const uint2 w, float s) {
 // Rows slots[i], bound by HBM: `lanes` (16 or 32) lanes of a warp take one slot's
 // K and V rows, 8 codes a lane (8-byte loads, 16-byte stores, both without gaps),
 // up to four steps in flight.  16384 slots x 8 heads (100 MB, 15 us of traffic):
-// 28.3 us with a thread per 8 codes and 64-bit index divisions, 24.0 us with 16
-// codes a lane (its 16-byte stores leave gaps).
+// 15.2 us, 17.7 with slots in random order; 28.3 us with a thread per 8 codes and
+// 64-bit index divisions, 24.0 us with 16 codes a lane (its 16-byte stores leave gaps).
 constexpr int kLoadFlight = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
