@@ -340,3 +340,20 @@ def test_mixed_batch_in_place_with_padding(dtype):
     nvkv.paged_attention_fp8b(q, *args, out=q, **kw)
     torch.cuda.synchronize()
     assert torch.equal(q[:-5], out[:-5]) and torch.equal(q[-5:], before[-5:])
+
+
+@pytest.mark.parametrize("n,skew", [(148, 0), (200, 700), (296, 300), (296, 2500), (297, 300)])
+def test_about_as_many_sequences_as_shares(n, skew):
+    """One kv head: sequences that get a share each (equal or nearly), others that
+    are cut, empty ones among them, one more than the shares."""
+    rng = np.random.default_rng(n + skew)
+    k_lens = (300 + rng.integers(0, skew + 1, n)).tolist()
+    q_lens = (np.arange(n) % 11 != 3).astype(int).tolist()
+    pool, bt, rows = filled(k_lens, 1, P=128, seed=n)
+    q = _q(sum(q_lens) + 2, 4, torch.bfloat16, n)
+    out = torch.full_like(q, 7.0)
+    nvkv.paged_attention_fp8b(q, *pool, cu(q_lens), cu(k_lens), bt, 1, max(k_lens), D ** -0.5,
+                              out=out)
+    torch.cuda.synchronize()
+    assert nvkv.device_error() == 0 and bool((out[-2:] == 7).all())
+    check_attention(out, q, rows, q_lens, k_lens, D ** -0.5, SHORT)
