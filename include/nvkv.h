@@ -319,7 +319,8 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  *
  * nvkv_load_kvcache_fp8b: k_out / v_out [n, Hkv, 128] = dtype(code * scale) of
  * rows slots[i] (negative: zeros; past the pool: zeros, recorded).  f16
- * outputs saturate at 65504.
+ * outputs saturate at 65504.  Outputs that overlap each other or the pool are
+ * refused.
  *
  * nvkv_paged_attention_fp8b: nvkv_paged_attention over an fp8b pool (paged
  * only).  When max_seqlen_q * (Hq / Hkv) <= 32 every sequence runs on the
@@ -329,11 +330,11 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * the caller passes prompt_kv_tokens >= the sum of their k_len (a prompt that
  * does not fit is skipped and recorded as NVKV_DEVERR_SEQLEN).  Malformed
  * sequences are skipped and recorded as in nvkv_paged_attention.  max_seqlen_k
- * up to 2^30; out may be q when its rows are dense.  Products
- * are exact in the codes: queries enter as three e4m3 pieces (12 significant
- * bits), the softmax weights as four (2^-12 of a weight down to 2^-17 of the
- * row's largest), sums in f32.  Calls
- * that may overlap on the GPU need a workspace each.
+ * goes up to 2^30; out may be q when its rows are dense.  Products are exact in
+ * the codes: queries enter as three e4m3 pieces (12 significant bits), the
+ * softmax weights as four (2^-12 of a weight down to 2^-17 of the row's
+ * largest), sums in f32.  Calls that may overlap on the GPU need a workspace
+ * each.
  * ---------------------------------------------------------------------- */
 #define NVKV_FP8B_BLOCK 16 /* slots that share a scale */
 

@@ -515,7 +515,7 @@ def dequantize_pages_fp8(cache, scales) -> np.ndarray:
 # --------------------------------------------------------------------------
 # Rotary positions (any layout, part of the head, any frequencies) and the
 # block-scaled e4m3 pool: 16 slots and a kv head share a power-of-two scale.
-# No counterpart in the reference; the checker of nvkv_rope, nvkv_rope_append
+# No counterpart in the reference; the definition of nvkv_rope, nvkv_rope_append
 # and nvkv_paged_attention_fp8b, from the definitions in 64 bits.
 # --------------------------------------------------------------------------
 FP8B_BLOCK = 16
