@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256)
       for (int c0 = l; c0 < chunks; c0 += lanes * kLoadFlight) {
         uint2 k[kLoadFlight], v[kLoadFlight];
         float2 s[kLoadFlight];
-  #pragma unroll
+#pragma unroll
         for (int f = 0; f < kLoadFlight; ++f) {
           const int c = c0 + f * lanes;
           if (c < chunks) {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256)
             s[f] = *reinterpret_cast<const float2*>(sc + (c / (kBD / 8)) * per * 2);
           }
         }
-  #pragma unroll
+#pragma unroll
         for (int f = 0; f < kLoadFlight; ++f) {
           const int c = c0 + f * lanes;
           if (c < chunks) {
