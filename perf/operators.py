@@ -27,16 +27,12 @@ MIN_E = -100  # smallest scale exponent
 DT = {"bf16": torch.bfloat16, "f16": torch.float16}
 
 
-_loaded = []
-
-
 def _ops():
-    """The framework's calls, imported once as a user's program does."""
-    if not _loaded:
-        sys.path.insert(0, os.path.join(os.getcwd(), "nanovllm-rs_b200"))
-        from nvkv import ops
-        _loaded.append(ops)
-    return _loaded[0]
+    pkg = os.path.join(os.getcwd(), "nanovllm-rs_b200")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from nvkv import ops
+    return ops
 
 
 # ---------------------------------------------------------------------------
