@@ -244,6 +244,26 @@ __device__ __forceinline__ void pf_issue_pv(uint32_t d_tmem, uint32_t p_tmem, ui
   }
 }
 
+// Clears the rows `keys` .. 127 of the V tile in ring load t, thread r row r: rows
+// behind a sequence's last key belong to another sequence or were never written,
+// and a weight of 0 times a NaN or an infinity there would be NaN.  (Their scores
+// are masked.)  Ends with the writes ordered before the caller's arrive that lets
+// PV read the tile.  The load is at most one ring turn ahead of the phase that the
+// caller has seen (S of this tile is done, so the ring's loads t - 5 and before
+// are), so its parity is unambiguous.  False (warp-uniform) when the wait ran out.
+__device__ __forceinline__ bool pf_clear_behind(uint8_t* smem, uint64_t* kv_full, uint32_t t,
+                                                int keys, int r, int* err) {
+  const uint32_t s = t % kPfSlots;
+  if (!__all_sync(0xffffffffu, mbar_wait(&kv_full[s], (t / kPfSlots) & 1u, err))) return false;
+  if (r >= keys) {
+    uint4* row = reinterpret_cast<uint4*>(smem + kPfOffKV + s * kPfTile + r * 128);
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) row[c] = row[c + kPfHalf / 16] = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  return true;
+}
+
 // ---- work plan --------------------------------------------------------------
 // Checks one sequence's lengths against the buffers before anything is read
 // or written for it.  Returns its q tiles, 0 for a decode row (q_len <= 1,
@@ -696,6 +716,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           }
           tmem_wait_st();
           l += rs;
+          if (x == 0 && (j + 1) * kPfBN > it.k_len) {  // slot B's PV is issued behind this one's
+            if (!pf_clear_behind(smem, kv_full, 2 * g + 1, it.k_len - j * kPfBN, r, p.err)) {
+              alive = false;
+              break;
+            }
+          }
           tc_fence_before();
           mbar_arrive(&p_full[x]);
         }
