@@ -318,9 +318,10 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * other overlap of q_out, the inputs and the caches is refused.
  *
  * nvkv_load_kvcache_fp8b: k_out / v_out [n, Hkv, 128] = dtype(code * scale) of
- * rows slots[i] (negative: zeros; past the pool: zeros, recorded).  f16
- * outputs saturate at 65504.  Outputs that overlap each other or the pool are
- * refused.
+ * rows slots[i] (negative: zeros; past the pool: zeros, recorded).  Codes may
+ * round a value up past the dtype's range (65504 in f16 to 65536): such values
+ * become its largest one, here and in what the attention below reads and
+ * writes.  Outputs that overlap each other or the pool are refused.
  *
  * nvkv_paged_attention_fp8b: nvkv_paged_attention over an fp8b pool (paged
  * only).  When max_seqlen_q * (Hq / Hkv) <= 32 every sequence runs on the

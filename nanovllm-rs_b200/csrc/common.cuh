@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 #include <utility>
 
 #include "../../include/nvkv.h"
@@ -209,6 +210,16 @@ struct DT<__half> {
     return *reinterpret_cast<uint32_t*>(&h);
   }
 };
+
+// A finite result that the dtype cannot hold becomes its largest value, not an
+// infinity; NaN stays.  For rows of an e4m3 pool, whose codes hold no infinities but
+// may round a value up past the dtype's range.
+template <typename T>
+__device__ __forceinline__ float saturate(float x) {
+  const float top = std::is_same<T, __half>::value ? 65504.f
+                    : std::is_same<T, __nv_bfloat16>::value ? 0x1.fep127f : 0x1.fffffep127f;
+  return x != x ? x : fminf(fmaxf(x, -top), top);
+}
 
 // round-trip through the storage dtype (the reference rounds after each op)
 template <typename T>

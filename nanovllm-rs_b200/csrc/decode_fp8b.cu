@@ -827,11 +827,11 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
       if (whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < n) static_cast<T*>(p.out)[to[i]] = DT<T>::from_f(val[i]);
+          if (i < n) static_cast<T*>(p.out)[to[i]] = DT<T>::from_f(saturate<T>(val[i]));
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < n) p.ws_o[to[i]] = val[i];
+          if (i < n) p.ws_o[to[i]] = saturate<float>(val[i]);
       }
     }
     }
@@ -887,7 +887,8 @@ __global__ void __launch_bounds__(kBD) combine_fp8b_kernel(const Params p) {
     if (last || n < 32) break;
   }
   const int64_t at = (int64_t)(q0 + r / p.group) * p.hq + kvh * p.group + r % p.group;
-  static_cast<T*>(p.out)[at * kBD + threadIdx.x] = DT<T>::from_f(wsum == 0.f ? 0.f : acc / wsum);
+  static_cast<T*>(p.out)[at * kBD + threadIdx.x] =
+      DT<T>::from_f(saturate<T>(wsum == 0.f ? 0.f : acc / wsum));
 }
 
 int padded_rows(int rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }

@@ -26,15 +26,10 @@ __device__ __forceinline__ void e4m3x4_f32(uint32_t w, float* f) {
   f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
 }
 
-// two values of code * scale in the dtype; f16 saturates (a code's rounding may
-// have carried a value past 65504)
+// two values of code * scale in the dtype
 template <typename T>
 __device__ __forceinline__ uint32_t pack_value(float a, float b) {
-  if (std::is_same<T, __half>::value) {
-    a = a != a ? a : fminf(fmaxf(a, -65504.f), 65504.f);
-    b = b != b ? b : fminf(fmaxf(b, -65504.f), 65504.f);
-  }
-  return DT<T>::from_f2(a, b);
+  return DT<T>::from_f2(saturate<T>(a), saturate<T>(b));
 }
 
 // 8 codes times their scale -> 8 values.
