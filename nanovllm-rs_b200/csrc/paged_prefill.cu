@@ -12,7 +12,8 @@
 // persistent (one CTA per SM walking its work items, see pf_work).  10 warps:
 //   warp 0      TMA producer: Q_A/Q_B per item, then K_j, V_j (128 keys each,
 //               pages resolved through block_tables) through a 5-slot ring,
-//               SWIZZLE_128B, each CTA loading its own tiles;
+//               SWIZZLE_128B, each CTA loading its own tiles; in the V tile that
+//               holds a sequence's end it clears the rows behind the last key;
 //   warp 1      allocates all 512 TMEM columns (S_A, S_B, O_A, O_B) and
 //               issues every tcgen05.mma.cta_group::1.kind::f16 from one
 //               thread in the order  PV_A(j), S_A(j+1), PV_B(j), S_B(j+1),
@@ -56,7 +57,7 @@ constexpr int kPfOffQA = 0;
 constexpr int kPfOffQB = kPfOffQA + kPfTile;
 constexpr int kPfOffKV = kPfOffQB + kPfTile;
 constexpr int kPfOffBar = kPfOffKV + kPfSlots * kPfTile;
-constexpr int kPfNumBars = 2 + 2 * kPfSlots + 6;
+constexpr int kPfNumBars = 2 + 2 * kPfSlots + 7;
 constexpr int kPfSmemBytes = kPfOffBar + kPfNumBars * 8 + 16 + 1024;
 constexpr uint32_t kPfTmemCols = 512;
 constexpr int kPfCtas = 148;  // B200 SMs
@@ -242,26 +243,6 @@ __device__ __forceinline__ void pf_issue_pv(uint32_t d_tmem, uint32_t p_tmem, ui
     const uint64_t bd = sdesc(sv + kk * 16 * 128, kPfHalf, 1024);
     tc_mma_tmem_a(d_tmem, p_tmem + kk * 8, bd, idesc, (accumulate || kk > 0) ? 1u : 0u);
   }
-}
-
-// Clears the rows `keys` .. 127 of the V tile in ring load t, thread r row r: rows
-// behind a sequence's last key belong to another sequence or were never written,
-// and a weight of 0 times a NaN or an infinity there would be NaN.  (Their scores
-// are masked.)  Ends with the writes ordered before the caller's arrive that lets
-// PV read the tile.  The load is at most one ring turn ahead of the phase that the
-// caller has seen (S of this tile is done, so the ring's loads t - 5 and before
-// are), so its parity is unambiguous.  False (warp-uniform) when the wait ran out.
-__device__ __forceinline__ bool pf_clear_behind(uint8_t* smem, uint64_t* kv_full, uint32_t t,
-                                                int keys, int r, int* err) {
-  const uint32_t s = t % kPfSlots;
-  if (!__all_sync(0xffffffffu, mbar_wait(&kv_full[s], (t / kPfSlots) & 1u, err))) return false;
-  if (r >= keys) {
-    uint4* row = reinterpret_cast<uint4*>(smem + kPfOffKV + s * kPfTile + r * 128);
-#pragma unroll 1
-    for (int c = 0; c < 8; ++c) row[c] = row[c + kPfHalf / 16] = make_uint4(0, 0, 0, 0);
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  return true;
 }
 
 // ---- work plan --------------------------------------------------------------
@@ -482,7 +463,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   uint64_t* s_full = kv_empty + kPfSlots;   // [2]: S_x written by the MMA
   uint64_t* p_full = s_full + 2;            // [2]: S_x read, P_x written (O_x rescaled / read)
   uint64_t* o_done = p_full + 2;            // [2]: PV_x finished (O_x stable, P_x free)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* v_end = o_done + 2;             // a V tile that a sequence ends in has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_end + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nslot = p.pair ? 2 : 1;
@@ -499,6 +481,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&p_full[x], 128);
       mbar_init(&o_done[x], 1);
     }
+    mbar_init(v_end, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -513,33 +496,41 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 
   if (warp == 0) {
     // ------------------------------ TMA producer ------------------------------
+    // the whole warp walks the loop, lane 0 issues
     if (lane == 0) {
       tma_prefetch_desc(&tmap_q);
       tma_prefetch_desc(&tmap_k);
       tma_prefetch_desc(&tmap_v);
-      uint32_t nq = 0, t = 0;  // items loaded, K/V ring loads (running over items)
-      bool ok = true;
-      for (int k = 0; ok && (int64_t)k * gridDim.x < pf_num_items<kPlan>(p); ++k) {
-        const int w = pf_work(k);
-        PfItem it;
-        if (w >= pf_num_items<kPlan>(p) || !pf_item<kPlan>(p, w, it)) continue;
-        if (nq > 0 && !mbar_wait(q_empty, (nq - 1) & 1u, p.err)) break;
+    }
+    uint32_t nq = 0, t = 0, nv = 0;  // items loaded, K/V ring loads, V ends (running over items)
+    bool ok = true;
+    for (int k = 0; ok && (int64_t)k * gridDim.x < pf_num_items<kPlan>(p); ++k) {
+      const int w = pf_work(k);
+      PfItem it;
+      if (w >= pf_num_items<kPlan>(p) || !pf_item<kPlan>(p, w, it)) continue;
+      if (nq > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (nq - 1) & 1u, p.err))) break;
+      if (lane == 0) {
         mbar_arrive_expect_tx(q_full, nslot * kPfTile);
         for (int x = 0; x < nslot; ++x) {
           uint8_t* qd = smem + (x ? kPfOffQB : kPfOffQA);
           tma_load_3d(qd, &tmap_q, q_full, 0, it.head0 + x, (int)(it.qs + it.i0));
           tma_load_3d(qd + kPfHalf, &tmap_q, q_full, 64, it.head0 + x, (int)(it.qs + it.i0));
         }
-        ++nq;
-        for (int u = 0; u < 2 * it.ntiles; ++u, ++t) {  // K_0, V_0, K_1, V_1, ...
-          const int j = u >> 1;
-          const int s = (int)(t % kPfSlots);
-          const uint32_t ph = (t / kPfSlots) & 1u;
-          if (t >= kPfSlots && !mbar_wait(&kv_empty[s], ph ^ 1u, p.err)) {
-            ok = false;
-            break;
-          }
-          const int j0 = j * kPfBN;
+      }
+      ++nq;
+      for (int u = 0; u < 2 * it.ntiles; ++u, ++t) {  // K_0, V_0, K_1, V_1, ...
+        const int j = u >> 1;
+        const int s = (int)(t % kPfSlots);
+        const uint32_t ph = (t / kPfSlots) & 1u;
+        if (t >= kPfSlots && !__all_sync(0xffffffffu, mbar_wait(&kv_empty[s], ph ^ 1u, p.err))) {
+          ok = false;
+          break;
+        }
+        const int j0 = j * kPfBN;
+        const int keys = it.k_len - j0;  // of the sequence, from this tile on
+        const bool end = (u & 1) && keys < kPfBN;
+        uint8_t* dst = smem + kPfOffKV + s * kPfTile;
+        if (lane == 0) {
           int64_t row;
           if (p.block_tables) {
             uint32_t page = p.block_tables[(int64_t)it.b * p.bt_stride + j0 / p.page_size];
@@ -551,11 +542,30 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           } else {
             row = (int64_t)it.ks + j0;
           }
-          uint8_t* dst = smem + kPfOffKV + s * kPfTile;
           const CUtensorMap* map = (u & 1) ? &tmap_v : &tmap_k;
-          mbar_arrive_expect_tx(&kv_full[s], kPfTile);
-          tma_load_3d(dst, map, &kv_full[s], 0, it.kvh, (int)row);
-          tma_load_3d(dst + kPfHalf, map, &kv_full[s], 64, it.kvh, (int)row);
+          uint64_t* bar = end ? v_end : &kv_full[s];
+          mbar_arrive_expect_tx(bar, kPfTile);
+          tma_load_3d(dst, map, bar, 0, it.kvh, (int)row);
+          tma_load_3d(dst + kPfHalf, map, bar, 64, it.kvh, (int)row);
+        }
+        if (end) {
+          // Rows behind the last key belong to another sequence or were never
+          // written; a weight of 0 times a NaN or an infinity there would be NaN.
+          // (Their scores are masked.)  The consumers' barrier follows the clearing.
+          // Here, a tile or two ahead of its use, it costs nothing: 16 x 1024 prompts
+          // 199 us, 201 without it.  In the softmax warpgroups, whose registers are
+          // full, it took 207-213 us, ragged ends or not, by the issuing thread 214-219.
+          if (!__all_sync(0xffffffffu, mbar_wait(v_end, nv & 1u, p.err))) {
+            ok = false;
+            break;
+          }
+          ++nv;
+          for (int i = lane; i < (kPfBN - keys) * 16; i += 32)  // row keys + i / 16, 16 bytes each
+            *reinterpret_cast<uint4*>(dst + (i & 8 ? kPfHalf : 0) + (keys + (i >> 4)) * 128 +
+                                      (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[s]);
         }
       }
     }
@@ -716,12 +726,6 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           }
           tmem_wait_st();
           l += rs;
-          if (x == 0 && (j + 1) * kPfBN > it.k_len) {  // slot B's PV is issued behind this one's
-            if (!pf_clear_behind(smem, kv_full, 2 * g + 1, it.k_len - j * kPfBN, r, p.err)) {
-              alive = false;
-              break;
-            }
-          }
           tc_fence_before();
           mbar_arrive(&p_full[x]);
         }
@@ -733,6 +737,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : 0.f;
+        pf_item<kPlan>(p, pf_work(k), it);  // again: fewer registers live above (206 -> 199 us)
         T* dst = reinterpret_cast<T*>(p.out) +
                  ((int64_t)(it.qs + qi) * p.num_q_heads + it.head0 + x) * kPfD;
 #pragma unroll
