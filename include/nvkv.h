@@ -333,8 +333,9 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * sequences are skipped and recorded as in nvkv_paged_attention.  max_seqlen_k
  * goes up to 2^30; out may be q when its rows are dense.  Products are exact in
  * the codes: queries enter as three e4m3 pieces (12 significant bits), the
- * softmax weights as four (2^-12 of a weight down to 2^-17 of the row's
- * largest), sums in f32.  Calls that may overlap on the GPU need a workspace
+ * softmax weights times their values' scales as four (2^-12 of such a product
+ * down to 2^-17 of the row's largest), sums in f32; a key counts in the
+ * softmax's sum whatever its values' scale.  Calls that may overlap on the GPU need a workspace
  * each.
  * ---------------------------------------------------------------------- */
 #define NVKV_FP8B_BLOCK 16 /* slots that share a scale */

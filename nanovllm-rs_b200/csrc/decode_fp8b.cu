@@ -12,13 +12,24 @@
 // the columns are read.
 //
 // A compute thread owns one key of the tile (one TMEM lane) and up to 8 of its
-// rows: it joins its scores, multiplies by the key block's K scale, and forms z =
-// S + log2(V scale), so a weight 2^(z - M) already carries the value's scale and O
-// needs none; the row sum takes the scale back out (an exact power of two).  M is a
-// row's maximum of z over the CTA's keys, to within a headroom: one barrier with a
-// reduced flag a tile says whether any score has left it; only then are maxima
-// joined (redux.sync in a warp, shared memory over the four) and O rescaled in
-// TMEM.  Weights leave as 8- or 16-byte stores (N-major B operand).
+// rows: it joins its scores S, multiplies by the key block's K scale, and forms z =
+// S + ev, ev = log2(V scale), so a weight 2^(z - M) already carries the value's scale
+// and O needs none; the row sum takes the scale back out (an exact power of two).  M
+// is a row's maximum of z over the CTA's keys, to within a headroom: one barrier with
+// a reduced flag a tile says whether any score has left it; only then are maxima
+// joined (redux.sync in a warp, shared memory over the four) and O rescaled in TMEM.
+// Weights leave as 8- or 16-byte stores (N-major B operand).
+//
+// V scales may lie 2^220 apart (a block of zero values has the least one), and a key
+// whose z is 126 below M would be flushed to 0 before the row sum could take its scale
+// back out.  So the exponential of a key whose ev is more than kBelow below E, the
+// largest ev so far to within kAbove, is taken 2^d higher, d = E - kBelow - ev, and the
+// weight multiplied by 2^-d: weights are as before, and what the sum (in units of
+// 2^(M - E)) can lose is below 2^(kBelow + kAbove - 126) = 2^-62 of a row's largest.
+// The sum itself holds rows whose keys of large values weigh down to 2^-126 of the
+// others.  (A second maximum and exponential, of S alone, for every key: 16 rows 86
+// us against 80, 32 rows 82 against 77; a branch to them from the first tile that
+// needs it: 82 and 78.)
 //
 //   G warpgroups  compute, G = 1, or rows / 8 for 16 and 32 rows (a warp has TMEM
 //              lanes 32 (w % 4) ..): the chain of a tile, not its issue, sets their
@@ -41,12 +52,14 @@
 // as many as the shares and not far from equal, each is a share, uncut.
 //
 // Bound by HBM up to 8 rows: 2 x 128 bytes of codes + 0.5 of scales a key and kv
-// head.  256 sequences of ~1290 keys, 32 / 8 heads (681 MB): 114.8 us, 5.9 TB/s of
+// head.  256 sequences of ~1290 keys, 32 / 8 heads (681 MB): 115.1 us, 5.9 TB/s of
 // the 6.55 that a copy reaches; the same loads without products 96 us.  64 x 32768
-// keys, 8 / 1 heads: 90.2 us, 6.0 TB/s.  16 rows (64 x 2000 keys, 32 / 8 heads, 4
+// keys, 8 / 1 heads: 90.4 us, 6.0 TB/s.  16 rows (64 x 2000 keys, 32 / 8 heads, 4
 // queries each, 267 MB): 80 us, bound by the tile's chain of scores, weights and the
 // issue of 8 products; one warpgroup for all 16 rows took 87, and 2 CTAs of 2 stages
 // instead of one of 6 then 85 (but 31.5 against 30.6 at 64 x 3000 keys of one head).
+#include <float.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -74,7 +87,10 @@ constexpr float kPiece1 = 1.f / 32.f, kPiece2 = 1.f / 1024.f, kPiece3 = 1.f / 32
 // and 8 rows, keep 9 bits at 2^-15: too few where one key takes nearly all of the
 // weight and the answer lies in the others.)
 constexpr float kHeadroom = 3.f;
-constexpr float kWeight = 32.f;
+constexpr int kWeightLog2 = 5;
+// Maxima of no keys yet: finite, so that the score of a hidden key, -inf, less it is -inf.
+constexpr float kNoMax = -3e38f;
+constexpr int kBelow = 48, kAbove = 16;
 
 // Rows a CTA serves, padded: 4, 8, 16 or 32; its resources by that.
 template <int HP>
@@ -260,6 +276,7 @@ __device__ __forceinline__ bool bar_compute_any(int g, bool flag) {
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ float redux_max(float x) {
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
@@ -376,6 +393,7 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
   __shared__ int64_t sums[kThreads / 32];
   __shared__ int tops[kThreads / 32];
   __shared__ int start_b, start_t;
+  __shared__ int4 top_ev[C::kGroups];  // the four warps' largest ev
 
   const int cta = blockIdx.x, share = cta / p.hkv, kvh = cta % p.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -630,11 +648,12 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
     float M[R], l[R], rf_r[R];  // (unused rows: no score passes infinity, every weight is 0)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      M[r] = r0 + r < rows ? -INFINITY : INFINITY;
+      M[r] = r0 + r < rows ? kNoMax : INFINITY;
       l[r] = 0.f;
       rf_r[r] = rowf[qb * HP + r0 + r];
     }
     const int seen = p.causal ? k_len - sq_info.q_len + 1 : k_len;  // keys that every row sees
+    int E = -100;
     for (int i = 0; i < n_tiles; ++i, ++it) {
       const int s = st, x = it & 1;
       alive = alive && mbar_ready(&s_full[x], (it >> 1) & 1, p.err) &&
@@ -645,11 +664,13 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
       const float2 sc = *reinterpret_cast<const float2*>(ssc + s * kBScale +
                                                          key / NVKV_FP8B_BLOCK * 2);
       const float ks = sc.x;
-      // log2 of the V scale, a power of two (a cleared pool's 0 counts as the least;
-      // the upper bound keeps a stale block's NaN out of the masked sums)
-      const int ev = min(max((int)(__float_as_uint(sc.y) >> 23 & 0xffu) - 127, -100), 120);
+      // log2 of the V scale, a power of two (a cleared pool's 0 counts as the least; a
+      // key past the end may have a stale block's)
       const int j = (cur.t + i) * kBTile + key;
-      float z[R];
+      const int ev = j < k_len ? min(max((int)(__float_as_uint(sc.y) >> 23 & 0xffu) - 127, -100), 120)
+                               : E;
+      int d = max(E - kBelow - ev, 0);
+      float z[R];  // (+ d)
       const uint32_t cs = lane_addr + x * kCols + r0;
       if constexpr (R == 4) {
         float a[16];
@@ -668,25 +689,30 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
         for (int r = 0; r < 8; ++r)
           z[r] = a0[r] + a1[r] * kPiece1 + a2[r] * kPiece2;
       }
-      bool over = false;  // a score past its row's headroom
+      float top = ev > E + kAbove ? INFINITY : -INFINITY;
 #pragma unroll
-      for (int r = 0; r < R; ++r) z[r] = z[r] * (rf_r[r] * ks) + (float)ev;
+      for (int r = 0; r < R; ++r) z[r] = z[r] * (rf_r[r] * ks) + (float)(ev + d);
       if ((cur.t + i + 1) * kBTile > seen) {
 #pragma unroll
         for (int r = 0; r < R; ++r) z[r] = j <= rowlim[r0 + r] ? z[r] : -INFINITY;
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) over |= z[r] > M[r] + kHeadroom;
-      if (bar_compute_any(grp, over)) {
+      for (int r = 0; r < R; ++r) top = fmaxf(top, z[r] - M[r]);
+      if (bar_compute_any(grp, top > kHeadroom)) {
         // new maxima: of the warp's keys, lane r keeping row r's, then of the four warps'
         float mine = -INFINITY;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float m = redux_max(z[r]);
+          const float m = redux_max(z[r] - (float)d);
           if (lane == r) mine = m;
         }
         if (lane < R) red[wg * HP + r0 + lane] = mine;
+        const int top = __reduce_max_sync(0xffffffffu, ev);
+        if (lane == 0) reinterpret_cast<int*>(&top_ev[grp])[wg] = top;
         bar_compute(grp);
+        const int4 te = top_ev[grp];
+        const int up_e = max(max(max(te.x, te.y), max(te.z, te.w)) - E, 0);
+        const float fac_e = ex2_mufu((float)min(up_e, 126));
         float fac[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -694,14 +720,19 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
           const float m = fmaxf(fmaxf(x[0], x[HP]), fmaxf(x[2 * HP], x[3 * HP]));
           const bool up = m > M[r] + kHeadroom;
           fac[r] = up ? ex2_mufu(M[r] - m) : 1.f;
+          l[r] *= up ? ex2_mufu(M[r] - m + (float)up_e) : fac_e;
           M[r] = up ? m : M[r];
-          l[r] *= fac[r];
         }
+        E += up_e;
+        const int more = max(E - kBelow - ev, 0) - d;
+        d += more;
+#pragma unroll
+        for (int r = 0; r < R; ++r) z[r] += (float)more;
         bar_compute(grp);  // (the next exchange may be the next tile's)
         if (i > 0) {  // O is in units of 2^M
           alive = alive && mbar_ready(&o_done[x ^ 1], ((it - 1) >> 1) & 1, p.err);
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int pc = 0; pc < kPPieces; ++pc) {
             const uint32_t a = lane_addr + 2 * kCols + pc * HP + r0;
             float o[R];
@@ -726,17 +757,16 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
         }
       }
       // weights, scaled for the pieces; the row sums without the V scale
-      const float unscale = __uint_as_float((uint32_t)(127 - ev) << 23);
+      const float unscale = pow2(E - ev - d), weight = pow2(max(kWeightLog2 - d, -126));
       uint32_t w[kPPieces * R / 4];
 #pragma unroll
       for (int c = 0; c < R; c += 4) {
         float e[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float m = M[c + r] == -INFINITY ? 0.f : M[c + r];
-          e[r] = ex2_mufu(z[c + r] - m);
+          e[r] = ex2_mufu(z[c + r] - M[c + r]);
           l[c + r] += e[r] * unscale;
-          e[r] *= kWeight;
+          e[r] *= weight;
         }
         uint32_t pw[kPPieces];
         pieces4(e[0], e[1], e[2], e[3], pw);
@@ -794,8 +824,9 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
     if (!whole && threadIdx.x == 0)
       p.ws_desc[slot] = make_int2(alive ? cur.b : -1, cur.t + n_tiles == sq_info.tiles);
     const int r_ = r0 + lane % R;
-    const float ls = red[r_] + red[HP + r_] + red[2 * HP + r_] + red[3 * HP + r_];
-    const float inv = ls == 0.f ? 0.f : 1.f / (ls * kWeight);
+    float ls = red[r_] + red[HP + r_] + red[2 * HP + r_] + red[3 * HP + r_];
+    ls = ls > FLT_MAX ? FLT_MAX : ls;
+    const float inv = ls == 0.f ? 0.f : pow2(E - kWeightLog2) / ls;
     int64_t at = (int64_t)slot * (p.q_cap * p.group) + r_;
     if (whole) {
       at = (int64_t)(q0 + r_ / p.group) * p.hq + kvh * p.group + r_ % p.group;
@@ -803,7 +834,7 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
       float Mr = -INFINITY;
 #pragma unroll
       for (int r = 0; r < R; ++r) Mr = r == lane ? M[r] : Mr;
-      p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr + log2f(ls);
+      p.ws_lse[at] = ls == 0.f ? -INFINITY : Mr - (float)E + log2f(ls);
     }
     // four rows a step, their chains side by side; not unrolled, as this runs once a
     // part and mostly from a cold instruction cache
