@@ -250,7 +250,7 @@ int nvkv_paged_attention_fp8(const void* q, int64_t q_stride, int64_t num_q_toke
  * f32 arithmetic, rounded once.  positions [T] int64, any sign: negated
  * positions rotate back (with a = 1 the transposed rotation).  inv_freq: f64
  * [rot_dim / 2] on the device.  An output may be its own input (same pointer
- * and stride); any other overlap is refused.  rot_dim even, <= head_dim <=
+ * and stride); any other overlap of an output is refused.  rot_dim even, <= head_dim <=
  * 1024.
  * ---------------------------------------------------------------------- */
 #define NVKV_ROPE_PLAIN 0
@@ -315,13 +315,14 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  *   (no other block does).
  * q/k/v: [T, H, 128] with token strides (elements, multiples of 4), rows
  * 8-byte aligned; num_q_heads may be 0 (q, q_out NULL).  q_out may be q; any
- * other overlap of q_out, the inputs and the caches is refused.
+ * other overlap of what is written (q_out, the caches, the scales) with another
+ * buffer of the call is refused.
  *
  * nvkv_load_kvcache_fp8b: k_out / v_out [n, Hkv, 128] = dtype(code * scale) of
  * rows slots[i] (negative: zeros; past the pool: zeros, recorded).  Codes may
  * round a value up past the dtype's range (65504 in f16 to 65536): such values
  * become its largest one, here and in what the attention below reads and
- * writes.  Outputs that overlap each other or the pool are refused.
+ * writes.  Outputs that overlap each other, the pool or the slots are refused.
  *
  * nvkv_paged_attention_fp8b: nvkv_paged_attention over an fp8b pool (paged
  * only).  When max_seqlen_q * (Hq / Hkv) <= 32 every sequence runs on the
@@ -331,7 +332,8 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * the caller passes prompt_kv_tokens >= the sum of their k_len (a prompt that
  * does not fit is skipped and recorded as NVKV_DEVERR_SEQLEN).  Malformed
  * sequences are skipped and recorded as in nvkv_paged_attention.  max_seqlen_k
- * goes up to 2^30; out may be q when its rows are dense.  Products are exact in
+ * goes up to 2^30; out may be q when its rows are dense (any other overlap of
+ * out or the workspace is refused).  Products are exact in
  * the codes: queries enter as three e4m3 pieces (12 significant bits), the
  * softmax weights times their values' scales as four (2^-12 of such a product
  * down to 2^-17 of the row's largest), sums in f32; a key counts in the

@@ -14,6 +14,7 @@
 #include <cudaTypedefs.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <string>
 #include <type_traits>
 #include <utility>
@@ -71,6 +72,18 @@ bool rows_clash(const void* a, int64_t a_stride, int64_t a_row, const void* b, i
 inline bool spans_meet(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
+// Whether a buffer that a call writes shares memory with one of its other buffers
+// (null ones do not count).
+struct Span {
+  const void* p;
+  uint64_t bytes;
+};
+inline bool spans_meet(const void* a, uint64_t a_bytes, std::initializer_list<Span> others) {
+  for (const Span& o : others)
+    if (spans_meet(a, a_bytes, o.p, o.bytes)) return true;
+  return false;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

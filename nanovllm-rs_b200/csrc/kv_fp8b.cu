@@ -210,9 +210,11 @@ extern "C" int nvkv_load_kvcache_fp8b(const void* k_cache, const void* v_cache,
   bool meet = spans_meet(k_out, out_bytes, v_out, out_bytes);
   for (const void* o : {k_out, v_out})
     meet |= spans_meet(o, out_bytes, k_cache, pool) || spans_meet(o, out_bytes, v_cache, pool) ||
-            spans_meet(o, out_bytes, kv_scale, pool / (kBBlock * kBD) * 8);
+            spans_meet(o, out_bytes, kv_scale, pool / (kBBlock * kBD) * 8) ||
+            spans_meet(o, out_bytes, slots, (uint64_t)num_slots * 8);
   if (meet)
-    return set_error(NVKV_ERR_INVALID_ARG, "load_kvcache_fp8b: an output overlaps another or the pool");
+    return set_error(NVKV_ERR_INVALID_ARG,
+                     "load_kvcache_fp8b: an output overlaps another, the pool or the slots");
   const int lanes = num_kv_heads == 1 ? 16 : 32;  // 16 chunks of 8 codes a head
   const int64_t rows = 256 / lanes;                // a CTA's
   const unsigned blocks = (unsigned)std::min<int64_t>((num_slots + rows - 1) / rows, 148 * 16);
@@ -303,6 +305,18 @@ extern "C" int nvkv_paged_attention_fp8b(
   if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
     return set_error(NVKV_ERR_WORKSPACE, "paged_attention_fp8b: workspace missing or too small "
                                          "(need " + std::to_string(L.total) + " bytes)");
+  const uint64_t pool = (uint64_t)num_blocks * page_size * num_kv_heads * kBD;
+  const uint64_t cu_bytes = ((uint64_t)num_seqs + 1) * 4, out_bytes = (uint64_t)num_q_tokens * q_row * 2;
+  const Span kc = {k_cache, pool}, vc = {v_cache, pool}, sc = {kv_scale, pool / (kBBlock * kBD) * 8};
+  const Span cq = {cu_seqlens_q, cu_bytes}, ck = {cu_seqlens_k, cu_bytes};
+  const Span bt = {block_tables, ((uint64_t)(num_seqs - 1) * block_table_stride +
+                                  ((int64_t)max_seqlen_k + page_size - 1) / page_size) * 4};
+  if (spans_meet(out, out_bytes, {kc, vc, sc, cq, ck, bt}))
+    return set_error(NVKV_ERR_INVALID_ARG, "paged_attention_fp8b: out overlaps the pool or metadata");
+  if (spans_meet(workspace, L.total,
+                 {{q, (uint64_t)((num_q_tokens - 1) * q_stride + q_row) * 2}, {out, out_bytes}, kc, vc,
+                  sc, cq, ck, bt}))
+    return set_error(NVKV_ERR_INVALID_ARG, "paged_attention_fp8b: the workspace overlaps a buffer");
   AttnArgs a;
   a.q = q;
   a.q_stride = q_stride;

@@ -248,6 +248,10 @@ extern "C" int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t
       rows_clash(k_out, k_out_stride, kr, q, q_stride, qr, num_tokens) ||
       rows_clash(q_out, q_out_stride, qr, k_out, k_out_stride, kr, num_tokens))
     return set_error(NVKV_ERR_INVALID_ARG, "rope: q's and k's rows overlap");
+  const Span pos = {positions, (uint64_t)num_tokens * 8}, freq = {inv_freq, (uint64_t)rot_dim * 4};
+  if (spans_meet(q_out, (uint64_t)((num_tokens - 1) * q_out_stride + qr) * 2, {pos, freq}) ||
+      spans_meet(k_out, (uint64_t)((num_tokens - 1) * k_out_stride + kr) * 2, {pos, freq}))
+    return set_error(NVKV_ERR_INVALID_ARG, "rope: an output overlaps positions or inv_freq");
   RopeParams p;
   p.q = q;
   p.k = k;

@@ -664,12 +664,22 @@ extern "C" int nvkv_rope_append(const void* q, int64_t q_stride, const void* k, 
   const uint64_t k_bytes = (uint64_t)((num_tokens - 1) * k_stride + kr) * 2;
   const uint64_t v_bytes = (uint64_t)((num_tokens - 1) * v_stride + kr) * 2;
   const uint64_t q_bytes = q ? (uint64_t)((num_tokens - 1) * q_stride + qr) * 2 : 0;
-  for (const void* c : {(const void*)k_cache, (const void*)v_cache})
-    if (spans_meet(c, pool, k, k_bytes) || spans_meet(c, pool, v, v_bytes) ||
-        spans_meet(c, pool, q, q_bytes) || spans_meet(c, pool, q_out, num_tokens * qr * 2))
-      return set_error(NVKV_ERR_INVALID_ARG, "rope_append: an input or q_out overlaps a cache");
-  if (spans_meet(k_cache, pool, v_cache, pool))
-    return set_error(NVKV_ERR_INVALID_ARG, "rope_append: k_cache and v_cache overlap");
+  const uint64_t scales = pool / (kApBlock * kApD) * 8, qo_bytes = (uint64_t)num_tokens * qr * 2;
+  const Span pos = {positions, (uint64_t)num_tokens * 8}, freq = {inv_freq, (uint64_t)rot_dim * 4};
+  const Span slot = {slot_mapping, (uint64_t)num_tokens * 8};
+  const Span qw = {q_norm_w, kApD * 2}, kw = {k_norm_w, kApD * 2};
+  // what the call writes: q_out (whose own input rows are checked above), the caches
+  // and the scales
+  if (spans_meet(q_out, qo_bytes, {pos, freq, slot, qw, kw}))
+    return set_error(NVKV_ERR_INVALID_ARG, "rope_append: q_out overlaps metadata or weights");
+  for (const Span& w : {Span{k_cache, pool}, Span{v_cache, pool}, Span{kv_scale, scales}})
+    if (spans_meet(w.p, w.bytes, {{q, q_bytes}, {k, k_bytes}, {v, v_bytes}, {q_out, qo_bytes}, pos,
+                                  freq, slot, qw, kw}))
+      return set_error(NVKV_ERR_INVALID_ARG,
+                       "rope_append: an input or q_out overlaps a cache or its scales");
+  if (spans_meet(k_cache, pool, v_cache, pool) ||
+      spans_meet(kv_scale, scales, {{k_cache, pool}, {v_cache, pool}}))
+    return set_error(NVKV_ERR_INVALID_ARG, "rope_append: k_cache, v_cache and kv_scale overlap");
   AppendParams p;
   p.q = q;
   p.k = k;
