@@ -194,7 +194,7 @@ extern "C" int nvkv_load_kvcache_fp8b(const void* k_cache, const void* v_cache,
     return set_error(NVKV_ERR_UNSUPPORTED, "load_kvcache_fp8b: output dtype must be bf16/f16");
   if (head_dim != kBD) return set_error(NVKV_ERR_UNSUPPORTED, "load_kvcache_fp8b: head_dim 128");
   if (num_slots < 0 || num_kv_heads <= 0 || num_kv_heads > 65536 || num_blocks <= 0 ||
-      page_size <= 0)
+      page_size <= 0 || num_blocks > INT64_MAX / page_size / ((int64_t)num_kv_heads * kBD))
     return set_error(NVKV_ERR_INVALID_ARG, "load_kvcache_fp8b: bad sizes");
   if (page_size % kBBlock)
     return set_error(NVKV_ERR_UNSUPPORTED, "load_kvcache_fp8b: page_size must be a multiple of 16");

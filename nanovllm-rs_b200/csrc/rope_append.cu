@@ -635,7 +635,8 @@ extern "C" int nvkv_rope_append(const void* q, int64_t q_stride, const void* k, 
   if (rot_dim <= 0 || rot_dim > kApD || rot_dim % 8)
     return set_error(NVKV_ERR_UNSUPPORTED, "rope_append: rot_dim must be a multiple of 8 up to 128");
   if (num_tokens < 0 || num_q_heads < 0 || num_kv_heads <= 0 || num_q_heads > 65536 ||
-      num_kv_heads > 65536 || num_blocks <= 0 || page_size <= 0)
+      num_kv_heads > 65536 || num_blocks <= 0 || page_size <= 0 ||
+      num_blocks > INT64_MAX / page_size / ((int64_t)num_kv_heads * kApD * 2))
     return set_error(NVKV_ERR_INVALID_ARG, "rope_append: bad sizes");
   if (kv_scale && page_size % kApBlock)
     return set_error(NVKV_ERR_UNSUPPORTED, "rope_append: page_size must be a multiple of 16");

@@ -37,6 +37,13 @@ def test_append_output_over_metadata(kw):
     assert _append(**kw) == ERR_INVALID_ARG
 
 
+@pytest.mark.parametrize("nb", [1 << 61, (1 << 63) - 1, (1 << 63) // (256 * 256) + 1])
+def test_pool_sizes_past_64_bits(nb):
+    assert _append(nb=nb) == ERR_INVALID_ARG
+    assert lib.nvkv_load_kvcache_fp8b(P(BIG), P(BIG), P(2 * BIG), P(3 * BIG), 4, 2, 128, nb, 256,
+                                      P(4 * BIG), P(5 * BIG), 1, None) == ERR_INVALID_ARG
+
+
 def test_load_output_over_slots():
     assert lib.nvkv_load_kvcache_fp8b(P(BIG), P(BIG), P(2 * BIG), P(3 * BIG), 4, 2, 128, 4, 256,
                                       P(4 * BIG), P(3 * BIG + 16), 1, None) == ERR_INVALID_ARG
