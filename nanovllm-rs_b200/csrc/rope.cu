@@ -175,8 +175,9 @@ extern "C" int nvkv_rope_frequencies(int rot_dim, double theta, const nvkv_rope_
   if (type == NVKV_ROPE_NTK && rot_dim > 2) base = theta * pow(f, rot_dim / (double)(rot_dim - 2));
   if (type == NVKV_ROPE_YARN) {
     const double bf = scaling->beta_fast, bs = scaling->beta_slow;
-    if (!(bf >= bs && bs > 0.0) || theta == 1.0)
-      return set_error(NVKV_ERR_INVALID_ARG, "rope_frequencies: beta_fast >= beta_slow > 0");
+    if (!(bf >= bs && bs > 0.0) || theta <= 1.0)
+      return set_error(NVKV_ERR_INVALID_ARG,
+                       "rope_frequencies: YARN needs beta_fast >= beta_slow > 0 and theta > 1");
     // the pair that makes `turns` turns over the original context
     auto pair_of = [&](double turns) {
       return rot_dim * log(orig / (turns * two_pi)) / (2.0 * log(theta));

@@ -73,3 +73,13 @@ POOL = 8 * 256 * 2 * 128  # bytes of a cache
 def test_attention_output_or_workspace_over_inputs(kw):
     assert _attend(**kw) == ERR_INVALID_ARG
     assert lib.nvkv_last_error()
+
+
+@pytest.mark.parametrize("theta", [1.0, 0.5])
+def test_yarn_needs_falling_frequencies(theta):
+    """Its ramp runs from fast pairs to slow ones: theta <= 1 has none."""
+    out = (ctypes.c_double * 32)()
+    a = ctypes.c_double()
+    sc = nvkv._lib.RopeScaling(nvkv._lib.ROPE_YARN, 4.0, 4096, 32.0, 1.0, 1.0, 4.0, 0.0)
+    assert lib.nvkv_rope_frequencies(64, theta, ctypes.byref(sc), out,
+                                     ctypes.byref(a)) == ERR_INVALID_ARG
