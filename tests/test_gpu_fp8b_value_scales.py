@@ -12,7 +12,7 @@ import torch
 
 import nvkv
 import nvkv_oracle as O
-from fp8b import D, G, check_attention, empty_pool, slots_of, tables
+from fp8b import D, G, attend64, check_attention, empty_pool, filled, slots_of, tables
 from helpers import cu
 from nvkv import ops
 
@@ -113,3 +113,32 @@ def test_sink_of_zero_values(L, hq, first, lead):
     q = torch.full((1, hq, D), lead / 8 / LOG2E / D ** 0.5).bfloat16().cuda()
     pool, bt, rows = _pool(k.bfloat16(), v.bfloat16(), hkv, seed=L)
     check_attention(_attend(q, pool, bt, L), q, [rows], [1], [L], D ** -0.5, 2.0 ** -11)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_gain,k_gain,v_gain", [(8.0, 1.0, 1.0), (1e-3, 1e3, 1e-4),
+                                                  (1.0, 1.0, 3e4), (30.0, 1.0, 1e-30)])
+def test_peaked_softmaxes_and_far_ranges(q_gain, k_gain, v_gain, dtype):
+    """Scores of a few hundred, keys and values far from 1; what is compared is what
+    the kernel wrote, with no term but its one rounding and the weights'.  A score of
+    up to 400 in the exponent is joined from three pieces' products in four steps
+    each: 16 roundings of 2^-24 x 400 are 2^-11.4 of a weight; weights keep 2^-12: 2^-10
+    covers them."""
+    if dtype == torch.float16 and not 1e-4 <= v_gain <= 1e3:
+        v_gain = 1e-3 if v_gain < 1 else 50.0  # (f16 holds up to 65504)
+    k_lens = [1, 100, 1300, 4000]
+    hq, hkv = 8, 2
+    g = torch.Generator().manual_seed(12)
+    q = (torch.randn(4, hq, D, generator=g) * q_gain).to(dtype).cuda()
+    if dtype == torch.float16 and k_gain > 100:
+        k_gain = 100.0
+    pool, bt, rows = filled(k_lens, hkv, seed=11, dtype=dtype, k_gain=k_gain, v_gain=v_gain)
+    out = nvkv.paged_attention_fp8b(q, *pool, cu([1] * 4), cu(k_lens), bt, 1, 4000, D ** -0.5)
+    torch.cuda.synchronize()
+    assert nvkv.device_error() == 0
+    got, qn = out.double().cpu().numpy(), q.double().cpu().numpy()
+    f = torch.finfo(dtype)
+    for b in range(4):
+        want, bound = attend64(qn[b:b + 1], *rows[b], D ** -0.5)
+        tol = abs(want) * f.eps / 2 * (1 + 2.0 ** -10) + bound * 2.0 ** -10 + f.smallest_normal * f.eps
+        assert (abs(got[b:b + 1] - want) <= tol).all(), k_lens[b]
