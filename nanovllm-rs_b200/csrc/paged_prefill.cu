@@ -552,9 +552,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           // Rows behind the last key belong to another sequence or were never
           // written; a weight of 0 times a NaN or an infinity there would be NaN.
           // (Their scores are masked.)  The consumers' barrier follows the clearing.
-          // Here, a tile or two ahead of its use, it costs nothing: 16 x 1024 prompts
-          // 199 us, 201 without it.  In the softmax warpgroups, whose registers are
-          // full, it took 207-213 us, ragged ends or not, by the issuing thread 214-219.
+          // Here, a tile or two ahead of its use, it costs little: 120 decodes + 8 ragged
+          // prompts 268.5 us, 265.5 without it.  In the softmax warpgroups, whose registers
+          // are full, 16 x 1024 prompts took 207-213 us (199 now), ragged ends or not, by
+          // the issuing thread 214-219.
           if (!__all_sync(0xffffffffu, mbar_wait(v_end, nv & 1u, p.err))) {
             ok = false;
             break;
@@ -737,7 +738,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        pf_item<kPlan>(p, pf_work(k), it);  // again: fewer registers live above (206 -> 199 us)
+        // without a plan the item is read again, so that fewer registers are live above
+        // (206 -> 199 us); walking a plan's levels costs more than that gives
+        if (!kPlan) pf_item<kPlan>(p, pf_work(k), it);
         T* dst = reinterpret_cast<T*>(p.out) +
                  ((int64_t)(it.qs + qi) * p.num_q_heads + it.head0 + x) * kPfD;
 #pragma unroll
