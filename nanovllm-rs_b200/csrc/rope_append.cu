@@ -20,10 +20,14 @@
 // decode step (a CTA per token: latency), up to 16 for prompts.
 //
 // Least traffic for prompts: qkv read, q and codes written.  16 x 1024 tokens of
-// 32 + 8 + 8 heads (369 MB, 56 us): 89 us with norms, 83 without, 4.1-4.5 TB/s:
-// issue, the f64 of K among it.  A step of 256 tokens (10 MB): 5.5-6.2 us, the chain
-// of slot, kept rows, maximum and codes.  (K in f32 with an error bound, f64 where
-// it leaves a code undecided: 121 and 17 us; q and K / V in blocks of their own: 121.)
+// 32 + 8 + 8 heads (369 MB, 56 us): 89 us with norms, 83 without, 4.1-4.5 TB/s.  It
+// waits for rows: 80 registers leave 20 warps an SM, each of which loads its rows and
+// only then computes (half of the issue slots taken, f64 at 6 % of its pipe).  Up to
+// some 4700 tokens a window has 2 to 7 tokens and as many of the eight warps the q
+// rows: with norms 1184 tokens 24.6 us, 2400 28.2, 4096 33.6 (4.1, 8.3 and 14.1 us of
+// traffic).  A step of 256 tokens (10 MB): 5.5-6.2 us, the chain of slot, kept rows,
+// maximum and codes.  (K in f32 with an error bound, f64 where it leaves a code
+// undecided: 121 and 17 us; q and K / V in blocks of their own: 121.)
 #include <algorithm>
 #include <type_traits>
 
@@ -708,6 +712,11 @@ extern "C" int nvkv_rope_append(const void* q, int64_t q_stride, const void* k, 
   p.page = page_size;
   p.err = device_error_word();
   p.window = (int)std::min<int64_t>(kApMaxWindow, std::max<int64_t>(1, num_tokens / (148 * 4)));
+  // Two forms (see the kernel).  Block scales gain from two tokens a CTA on (32 + 8 + 8
+  // heads, norms, single tokens / windows: 1184 tokens 26.1 / 24.6 us, 2400 39.1 / 28.2),
+  // the dtype pool, whose warps then take whole tokens, from three (1184: 16.5 / 23.4,
+  // 1800: 24.6 / 24.7, 2400: 31.6 / 26.4).
+  if (!kv_scale && p.window < 3) p.window = 1;
   const int64_t ctas = (num_tokens + p.window - 1) / p.window;
   if (ctas > 0x7fffffffLL) return set_error(NVKV_ERR_INVALID_ARG, "rope_append: too many tokens");
   const size_t smem = (size_t)p.half * (p.window * sizeof(float2) +
