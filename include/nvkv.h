@@ -145,6 +145,9 @@ int nvkv_qknorm_rope(const void* qkv, int64_t qkv_stride, int64_t num_tokens, in
  * cu_seqlens_q/k: [num_seqs + 1] uint32 prefix sums (device memory).
  * Query i of sequence b (q_len = cu_q[b+1]-cu_q[b], k_len likewise) sees key
  * j iff j <= i + k_len - q_len when causal != 0 (all keys otherwise).
+ * Memory behind a sequence's last key is never seen, whatever it holds (NaN
+ * among it).  A NaN or an infinity in one of its own values may reach all of
+ * its query rows in that kv head, those whose mask hides the key among them.
  * Sequences with q_len == 1 run on the split-KV paged decode kernel
  * (TMA-staged K/V, warp-shuffle softmax, LSE combine); the others run on the
  * tcgen05 prefill kernel.  max_seqlen_q/k bound the per-sequence lengths.
@@ -291,7 +294,8 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  *   code, NaN stays NaN).
  * Because scales are powers of two, a block that a larger row joins is
  * re-encoded by shifting exponents: exact, but for codes that fall below
- * e4m3's normal range.
+ * e4m3's normal range.  Codes and scales start cleared to zero, unless every
+ * block is first entered at its first row.
  *
  * nvkv_rope_append: for each token t, in one launch,
  *   q' = norm(q), k' = norm(k)   (RMSNorm per head with q_norm_w / k_norm_w
@@ -333,12 +337,17 @@ int nvkv_rope(const void* q, int64_t q_stride, const void* k, int64_t k_stride, 
  * does not fit is skipped and recorded as NVKV_DEVERR_SEQLEN).  Malformed
  * sequences are skipped and recorded as in nvkv_paged_attention.  max_seqlen_k
  * goes up to 2^30; out may be q when its rows are dense (any other overlap of
- * out or the workspace is refused).  Products are exact in
- * the codes: queries enter as three e4m3 pieces (12 significant bits), the
- * softmax weights times their values' scales as four (2^-12 of such a product
- * down to 2^-17 of the row's largest), sums in f32; a key counts in the
- * softmax's sum whatever its values' scale.  Calls that may overlap on the GPU need a workspace
- * each.
+ * out or the workspace is refused).
+ * Decode kernel: products are exact in the codes; queries enter as three e4m3
+ * pieces (12 significant bits), the softmax weights times their values' scales
+ * as four (2^-12 of such a product down to 2^-17 of the row's largest), sums
+ * in f32; a key counts in the softmax's sum whatever its values' scale.
+ * Prefill kernel, as in nvkv_paged_attention: keys, values and softmax weights
+ * rounded to the dtype, some exponentials within 7.5e-5, sums in f32.  So one
+ * long sequence sends the short multi-token ones beside it there too, where
+ * they are less exact than in a call of their own and need workspace for
+ * their whole contexts.
+ * Calls that may overlap on the GPU need a workspace each.
  * ---------------------------------------------------------------------- */
 #define NVKV_FP8B_BLOCK 16 /* slots that share a scale */
 

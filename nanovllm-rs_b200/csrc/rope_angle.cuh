@@ -3,8 +3,10 @@
 // The angle of pair i at position p is p * inv_freq[i].  It is formed in 64
 // bits and reduced to a fraction of a turn there: at p = 10^5 an f32 product
 // is already 2^-8 radians off.  With f = inv_freq / 2 pi, the fraction r = p f
-// - rint(p f) lies in [-1/2, 1/2] and is off by at most |p f| 2^-52 turns,
-// below half an f32 ulp of 2 pi r up to |p| = 2^24.
+// - rint(p f) lies in [-1/2, 1/2].  Three roundings (1 / 2 pi, the two products)
+// put it off by at most 3 x 2^-53 of |p f|, so cos and sin inherit at most 3 x
+// 2^-53 |p inv_freq|: 2^-27 at |p| = 2^24 and inv_freq = 1, a quarter of half an
+// f32 ulp of 1.  The f32 form rounds r once more, 2^-24 of the reduced angle.
 #pragma once
 
 #include "common.cuh"
