@@ -52,15 +52,15 @@
 // as many as the shares and not far from equal, each is a share, uncut.
 //
 // Bound by HBM up to 8 rows where sequences are long: 2 x 128 bytes of codes + 0.5 of
-// scales a key and kv head.  256 sequences of ~1290 keys, 32 / 8 heads (681 MB): 115.1 us, 5.9 TB/s of
-// the 6.55 that a copy reaches; the same loads without products 96 us.  64 x 32768
-// keys, 8 / 1 heads: 90.4 us, 6.0 TB/s.  With 8 rows and 512-4096 keys (64 sequences,
-// 8 kv heads, 305 MB) 62.9 us, 4.8 TB/s: the tile's chain and the parts' ends show.  16
-// rows (64 x 2000 keys, 32 / 8 heads, 4 queries each, 267 MB): 80.5 us, bound by the
-// tile's chain of scores, weights and the issue of 8 products; 32 rows (32 / 4 heads,
-// 136 MB): 77.  Earlier forms at 16 rows: one warpgroup for all 87, and 2 CTAs of 2
-// stages instead of one of 6 then 85 (but 31.5 against 30.6 at 64 x 3000 keys of one
-// head).
+// scales a key and kv head.  256 sequences of ~1290 keys, 32 / 8 heads (681 MB): 115.1
+// us, 5.9 TB/s of the 6.55 that a copy reaches; the same loads without products 96 us.
+// 64 x 32768 keys, 8 / 1 heads: 90-91.5 us, 5.9-6.0 TB/s.  With 8 rows and 512-4096
+// keys (64 sequences, 8 kv heads, 305 MB) 62.9 us, 4.8 TB/s: the tile's chain and the
+// parts' ends show.  16 rows (64 x 2000 keys, 32 / 8 heads, 4 queries each, 267 MB):
+// 80.5 us, bound by the tile's chain of scores, weights and the issue of 8 products; 32
+// rows (32 / 4 heads, 136 MB): 77.  Earlier forms at 16 rows: one warpgroup for all 87,
+// and 2 CTAs of 2 stages instead of one of 6 then 85 (but 31.5 against 30.6 at 64 x
+// 3000 keys of one head).
 #include <float.h>
 
 #include <algorithm>
@@ -710,8 +710,8 @@ __global__ void __launch_bounds__(Cfg<HP>::kThreads, Cfg<HP>::kCtasPerSm)
           if (lane == r) mine = m;
         }
         if (lane < R) red[wg * HP + r0 + lane] = mine;
-        const int top = __reduce_max_sync(0xffffffffu, ev);
-        if (lane == 0) reinterpret_cast<int*>(&top_ev[grp])[wg] = top;
+        const int warp_ev = __reduce_max_sync(0xffffffffu, ev);
+        if (lane == 0) reinterpret_cast<int*>(&top_ev[grp])[wg] = warp_ev;
         bar_compute(grp);
         const int4 te = top_ev[grp];
         const int up_e = max(max(max(te.x, te.y), max(te.z, te.w)) - E, 0);
